@@ -5,6 +5,7 @@
 #include <climits>
 
 #include "../../include/hrm_ops.h"
+#include "abi_checks.h"
 #include "launch.h"
 
 namespace hrm {
@@ -27,28 +28,7 @@ int device_sm_count() {
 
 namespace {
 
-constexpr int kAbiVersion = 10000;  // 1.0.0
-
-int cuda_status(cudaError_t e) { return e == cudaSuccess ? HRM_OK : HRM_ERR_CUDA + (int)e; }
-
-// n * m for non-negative operands, or -1 when it would exceed limit.
-int64_t mul_checked(int64_t n, int64_t m, int64_t limit = INT64_MAX / 8) {
-  if (n < 0 || m < 0) return -1;
-  if (n != 0 && m > limit / n) return -1;
-  return n * m;
-}
-
-// True when [a, a + abytes) and [b, b + bbytes) share a byte.
-bool overlap(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
-  if (a == nullptr || b == nullptr || abytes <= 0 || bbytes <= 0) return false;
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-  return pa < pb + (uintptr_t)bbytes && pb < pa + (uintptr_t)abytes;
-}
-
-// Partial overlap (anything but identical ranges) of two equal-sized buffers.
-bool partial_overlap(const void* a, const void* b, int64_t bytes) { return a != b && overlap(a, bytes, b, bytes); }
-
-cudaStream_t as_cuda(hrm_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
+constexpr int kAbiVersion = 10100;  // 1.1.0
 
 }  // namespace
 
@@ -64,6 +44,7 @@ const char* hrm_status_string(int status) {
     case HRM_ERR_TABLE_RANGE: return "position_offset + seq_len exceeds the rope table";
     case HRM_ERR_DTYPE: return "unsupported dtype";
     case HRM_ERR_SCRATCH_LIMIT: return "request exceeds the fixed device scratch of an allocation-free entry point";
+    case HRM_ERR_ALIGNMENT: return "a pointer is not aligned as its entry point requires";
     default: break;
   }
   if (status > HRM_ERR_CUDA) return cudaGetErrorString(static_cast<cudaError_t>(status - HRM_ERR_CUDA));

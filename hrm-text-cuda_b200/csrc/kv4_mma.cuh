@@ -1,0 +1,72 @@
+// Warp-level helpers of the attention kernels over the 4-bit cache.
+#pragma once
+
+#include "kv4.cuh"
+
+namespace hrm {
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2^x, within 2 ulp; 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// D = A (16x16, row) * B (16x8, col) + D, bf16 operands, fp32 accumulators.
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// cp.async of BYTES (4, 8 or 16) global -> shared; zeros where !valid (src is not read then).
+template <int BYTES>
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? BYTES : 0;
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+// Query rows of one kv head up to which the probabilities are added to the
+// weights by the decode kernel itself (one block of rows holds them all).
+constexpr int64_t kDecodeRows = 8;
+// Query rows of one kv head up to which the decode kernel serves them, in blocks of 8.
+constexpr int64_t kChunkRows = 32;
+
+// What every attention kernel is given.
+struct AttnArgs {
+  const uint4* q;        // [batch, heads, seq, D] bf16
+  const uint16_t* gate;  // [batch, seq, heads, D] bf16, or null
+  uint16_t* out;         // [batch, seq, heads, D] bf16
+  Kv4View c;
+  int64_t batch, heads, kv_heads, group, seq;
+  int64_t cache_offset;
+  const int* cache_offsets;  // per sequence, or null
+  int64_t prefix_len;
+  float scale_log2;  // softmax scale * log2(e)
+  float* scores;  // weights wanted, rows of one block: [batch * kv_heads, rows, cache_len] scores (log2 units)
+  float* lse;     // weights wanted, more rows: [batch, heads, seq], log2 of each row's sum of 2^score
+};
+
+// Cache rows that query s of sequence b sees: [0, limit).
+__device__ __forceinline__ int visible_rows(const AttnArgs& a, int64_t b, int64_t s) {
+  const int64_t off = a.cache_offsets ? a.cache_offsets[b] : a.cache_offset;
+  int64_t lim = off + s + 1;
+  if (lim < a.prefix_len) lim = a.prefix_len;
+  if (lim > off + a.seq) lim = off + a.seq;
+  if (lim > a.c.cache_len) lim = a.c.cache_len;
+  return lim < 0 ? 0 : (int)lim;
+}
+
+// A word (S, Z) whose group reads back as NaN or an infinity.
+__device__ __forceinline__ bool kv4_not_finite(uint32_t sz) {
+  return (sz & 0x7f80u) == 0x7f80u || (sz & 0x7f800000u) == 0x7f800000u;
+}
+
+}  // namespace hrm

@@ -51,6 +51,33 @@ inline cudaError_t launch_kernel(void (*k)(KArgs...), int64_t grid, int block, s
   return cudaLaunchKernelEx(&cfg, k, static_cast<Args&&>(args)...);
 }
 
+// The same for thread-block clusters of `cluster` CTAs (grid a multiple of it).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_cluster(void (*k)(KArgs...), int64_t grid, int block, size_t smem, int cluster,
+                                  cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = HRM_PDL ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, static_cast<Args&&>(args)...);
+}
+
+// Lets kernel k be launched with `bytes` of dynamic shared memory on the current
+// device (needed above 48 KB).
+template <typename... KArgs>
+inline cudaError_t allow_shared(void (*k)(KArgs...), size_t bytes) {
+  return bytes <= 48 * 1024 ? cudaSuccess
+                            : cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
 cudaError_t launch_additive_inject(const void* a, const void* b, void* out, int64_t n, cudaStream_t s);
 cudaError_t launch_attn_gate(const void* gate, const void* attn, void* out, int64_t n, cudaStream_t s);
 cudaError_t launch_broadcast(void* dst, const void* src, int64_t n_copies, int64_t vec_len, cudaStream_t s);
@@ -77,6 +104,26 @@ cudaError_t launch_split_rope(const void* gqkv, void* gate, void* q, void* k, vo
 cudaError_t launch_rope_table(float* table, int64_t max_pos, int64_t head_dim, float theta, cudaStream_t s);
 
 cudaError_t launch_convert_to_bf16(const void* src, int dtype, void* dst, int64_t n, cudaStream_t s);
+
+struct Kv4View;
+struct AttnArgs;
+cudaError_t launch_split_rope_kv4(const void* gqkv, void* gate, void* q, void* k, void* v, const Kv4View& c,
+                                  int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
+                                  int64_t position_offset, const int* position_offsets, float theta,
+                                  const float* table, int64_t table_positions, int64_t cache_offset,
+                                  const int* cache_offsets, cudaStream_t s);
+cudaError_t launch_kv4_update(const void* k, const void* v, const Kv4View& c, int64_t batch, int64_t heads,
+                              int64_t seq, int64_t head_dim, int64_t position_offset, const int* position_offsets,
+                              int64_t cache_offset, const int* cache_offsets, cudaStream_t s);
+// `longest`: no sequence has more cache rows than this.
+cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s);
+cudaError_t launch_kv4_chunk(const AttnArgs& a, int64_t head_dim, cudaStream_t s);
+cudaError_t launch_kv4_weights(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s);
+// Whether the selection of `budget` out of at most n rows fits its shared memory.
+bool kv4_evict_fits(int64_t n, int64_t budget);
+cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_place, int64_t batch, int64_t kv_heads,
+                             int64_t head_dim, int64_t length, const int* lengths, int64_t budget,
+                             int64_t protect_from, const int* protect_froms, int* new_lengths, cudaStream_t s);
 
 // Bounded waits that ran out in the row kernels (device counter); reset sets it to 0.
 cudaError_t rownorm_wait_timeouts(unsigned int* count, bool reset);

@@ -5,6 +5,15 @@ package loads the library and fails loudly when it has not been built.
 """
 
 from ._lib import HrmError, LIB, LIB_PATH  # noqa: F401
+from .kv4 import (  # noqa: F401
+    Kv4Cache,
+    kv4_attention,
+    kv4_attention_workspace,
+    kv4_cache,
+    kv4_evict,
+    kv4_update,
+    split_gqkv_rope_kv4,
+)
 from .ops import (  # noqa: F401
     add_rms_norm,
     additive_inject,
@@ -40,4 +49,11 @@ __all__ = [
     "broadcast_vec",
     "convert_to_bf16",
     "wait_timeouts",
+    "Kv4Cache",
+    "kv4_cache",
+    "kv4_update",
+    "split_gqkv_rope_kv4",
+    "kv4_attention",
+    "kv4_attention_workspace",
+    "kv4_evict",
 ]

@@ -21,6 +21,7 @@ HRM_ERR_ALIASING = 4
 HRM_ERR_TABLE_RANGE = 5
 HRM_ERR_DTYPE = 6
 HRM_ERR_SCRATCH_LIMIT = 7
+HRM_ERR_ALIGNMENT = 8
 UPLOAD_STATIC_BYTES = 16 * 1024 * 1024  # HRM_UPLOAD_STATIC_BYTES
 DTYPES = {"bf16": 0, "f32": 1, "f16": 2}
 HRM_ERR_CUDA = 1000
@@ -28,6 +29,17 @@ HRM_ERR_CUDA = 1000
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+
+
+
+class Kv4CacheStruct(ctypes.Structure):
+    """hrm_kv4_cache."""
+
+    _fields_ = [("k_codes", _p), ("k_scales", _p), ("v_codes", _p), ("v_scales", _p), ("weights", _p),
+                ("positions", _p), ("batch", _i64), ("kv_heads", _i64), ("cache_len", _i64), ("head_dim", _i64)]
+
+
+_c = ctypes.POINTER(Kv4CacheStruct)
 
 # name -> argument types (every function returns int status).
 SIGNATURES = {
@@ -49,6 +61,11 @@ SIGNATURES = {
     "hrm_convert_to_bf16": [_p, ctypes.c_int, _p, _i64, _p],
     "hrm_upload_to_bf16": [_p, ctypes.c_int, _p, _i64, _p, _i64, _p],
     "hrm_upload_to_bf16_static": [_p, ctypes.c_int, _p, _i64, _p],
+    "hrm_kv4_update": [_c, _p, _p, _i64, _i64, _p, _i64, _p, _p],
+    "hrm_split_gqkv_rope_kv4": [_p, _p, _p, _p, _p, _c, _i64, _i64, _p, _f32, _p, _i64, _i64, _p, _p],
+    "hrm_kv4_attention": [_p, _c, _p, _p, _i64, _i64, _i64, _p, _i64, _f32, ctypes.c_int, _p, _i64, _p],
+    "hrm_kv4_attention_workspace": [_c, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)],
+    "hrm_kv4_evict": [_c, _c, _i64, _p, _i64, _i64, _p, _p, _p],
     "hrm_wait_timeouts": [ctypes.POINTER(ctypes.c_uint), ctypes.c_int],
     "hrm_abi_version": [],
 }

@@ -1,0 +1,236 @@
+"""The 4-bit KV cache: the buffers, the calls that write them, the attention that
+reads them and the eviction that bounds them (C ABI: the hrm_kv4_* entry points
+and hrm_split_gqkv_rope_kv4 of include/hrm_ops.h, where the format is defined).
+
+A decode loop with a bounded cache, one step:
+
+    gate, q, _, _ = split_gqkv_rope_kv4(gqkv, heads, cache, position, theta, table, cache_offset=rows, keep_kv=False)
+    o = kv4_attention(q, cache, rows, gate=gate, accumulate=True)     # [b, s, h, d], gated
+    rows = kv4_evict(cache, rows + s, budget, protect_from)           # int32 [b], back to at most budget
+
+Offsets and lengths are ints, or int32 CUDA tensors with one value per sequence
+(read on the device, so that a captured step can be replayed as they advance).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass, field
+from typing import Optional, Tuple, Union
+
+import torch
+
+from ._lib import Kv4CacheStruct, call
+from .ops import _launch, _need, _ptr
+
+GROUP = 32  # elements per (scale, base) pair
+HEAD_DIMS = (64, 128, 192, 256)
+
+Offset = Union[int, torch.Tensor]
+
+
+@dataclass
+class Kv4Cache:
+    """The buffers of one 4-bit cache (one layer's KV slot).
+
+    k_codes, v_codes   uint8 [batch, kv_heads, cache_len, head_dim / 2]
+    k_scales, v_scales bf16 [batch, kv_heads, cache_len, head_dim / 32, 2]
+    weights            fp32 [batch, kv_heads, cache_len], or None
+    positions          int32 [batch, kv_heads, cache_len], or None
+
+    The shapes are checked here, once; the calls then pass the buffers as they
+    are.  Do not resize or replace the tensors of a cache: make another one.
+    """
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    weights: Optional[torch.Tensor] = None
+    positions: Optional[torch.Tensor] = None
+    shape: Tuple[int, int, int, int] = field(init=False, repr=False)
+
+    def __post_init__(self):
+        _need(self.k_codes, "k_codes", (torch.uint8,))
+        if self.k_codes.dim() != 4 or 2 * self.k_codes.shape[3] not in HEAD_DIMS:
+            raise ValueError("k_codes must be [batch, kv_heads, cache_len, head_dim / 2], head_dim 64, 128, 192 or 256")
+        b, h, n, half = self.k_codes.shape
+        self.shape = (b, h, n, 2 * half)
+        want = {"v_codes": ((b, h, n, half), torch.uint8), "k_scales": ((b, h, n, 2 * half // GROUP, 2), torch.bfloat16),
+                "v_scales": ((b, h, n, 2 * half // GROUP, 2), torch.bfloat16), "weights": ((b, h, n), torch.float32),
+                "positions": ((b, h, n), torch.int32)}
+        for name, (shape, dtype) in want.items():
+            t = getattr(self, name)
+            if t is None and name in ("weights", "positions"):
+                continue
+            _need(t, name, (dtype,))
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+            if t.device != self.k_codes.device:
+                raise ValueError(f"{name} is on {t.device}, k_codes on {self.k_codes.device}")
+        ptr = [None if t is None else t.data_ptr()
+               for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.weights, self.positions)]
+        self._struct = Kv4CacheStruct(*ptr, b, h, n, 2 * half)
+        self._ref = ctypes.pointer(self._struct)
+
+
+def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, device=None, track: bool = False) -> Kv4Cache:
+    """A zeroed cache; track=True adds the weights and positions that kv4_evict needs."""
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim {head_dim}: the 4-bit cache takes {HEAD_DIMS}")
+    d = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+
+    def z(*tail, dtype):
+        return torch.zeros((batch, kv_heads, cache_len, *tail), dtype=dtype, device=d)
+
+    return Kv4Cache(z(head_dim // 2, dtype=torch.uint8), z(head_dim // GROUP, 2, dtype=torch.bfloat16),
+                    z(head_dim // 2, dtype=torch.uint8), z(head_dim // GROUP, 2, dtype=torch.bfloat16),
+                    z(dtype=torch.float32) if track else None, z(dtype=torch.int32) if track else None)
+
+
+def _offset(x: Offset, name: str, batch: int):
+    """(host value, tensor or None) of an int or an int32 CUDA tensor [batch]."""
+    if not isinstance(x, torch.Tensor):
+        return int(x), None
+    _need(x, name, (torch.int32,))
+    if x.numel() != batch:
+        raise ValueError(f"{name} must have one value per sequence ({batch}), got {x.numel()}")
+    return 0, x
+
+
+def kv4_update(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, position_offset: Offset = 0,
+               cache_offset: Offset = 0, *, stream=None) -> Kv4Cache:
+    """Writes k, v [batch, kv_heads, seq, head_dim] bf16 as cache rows cache_offset + s.
+
+    The rows' weights become 0 and their positions position_offset + s.  The
+    4-bit kv_cache_update (src/lib.rs:706-747).
+    """
+    _need(k, "k"); _need(v, "v")
+    b, h, _, d = cache.shape
+    if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (b, h, d):
+        raise ValueError(f"k and v must both be [{b}, {h}, seq, {d}]")
+    pos, pos_t = _offset(position_offset, "position_offset", b)
+    off, off_t = _offset(cache_offset, "cache_offset", b)
+    _launch("hrm_kv4_update", (k, v, cache.k_codes, pos_t, off_t), stream, cache._ref, _ptr(k), _ptr(v), k.shape[2], pos,
+            _ptr(pos_t), off, _ptr(off_t))
+    return cache
+
+
+def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, position_offset: Offset = 0,
+                        theta: float = 10000.0, table: Optional[torch.Tensor] = None, cache_offset: Offset = 0,
+                        out=None, keep_kv: bool = True, *, stream=None):
+    """split_gqkv_rope into a 4-bit cache: (gate [b, s, h, d], q, k, v [b, h, s, d]).
+
+    gate and q are split_gqkv_rope's; k and v are the values that the cache now
+    holds for these tokens (None with keep_kv=False).  `out`: the four buffers.
+    """
+    _need(gqkv, "gqkv")
+    b, h, _, d = cache.shape
+    if num_heads != h or gqkv.dim() != 3 or gqkv.shape[0] != b or gqkv.shape[2] != 4 * h * d:
+        raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
+    s = gqkv.shape[1]
+    if out is None:
+        new = lambda *shape: torch.empty(shape, dtype=gqkv.dtype, device=gqkv.device)  # noqa: E731
+        out = (new(b, s, h, d), new(b, h, s, d), new(b, h, s, d) if keep_kv else None,
+               new(b, h, s, d) if keep_kv else None)
+    for t, n in zip(out, ("gate", "q", "k", "v")):
+        if t is None and n in ("k", "v"):
+            continue
+        _need(t, n)
+        if t.numel() != b * s * h * d:
+            raise ValueError(f"{n} has the wrong size")
+    positions = 0
+    if table is not None:
+        _need(table, "table", (torch.float32,))
+        if table.dim() != 2 or table.shape[1] != d:
+            raise ValueError("table must be [positions, head_dim]")
+        positions = table.shape[0]
+    pos, pos_t = _offset(position_offset, "position_offset", b)
+    off, off_t = _offset(cache_offset, "cache_offset", b)
+    _launch("hrm_split_gqkv_rope_kv4", (gqkv, *out, cache.k_codes, table, pos_t, off_t), stream, _ptr(gqkv),
+            *(_ptr(t) for t in out), cache._ref, s, pos, _ptr(pos_t), theta, _ptr(table), positions, off, _ptr(off_t))
+    return tuple(out)
+
+
+def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gate: Optional[torch.Tensor] = None,
+                  prefix_len: int = 0, scale: Optional[float] = None, accumulate: bool = False,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                  stream=None) -> torch.Tensor:
+    """Attention of q [b, heads, s, d] over the cache; out [b, s, heads, d].
+
+    cache_offset counts the rows before the queries' own tokens, which the cache
+    already holds: query i sees rows j <= cache_offset + i, and those below
+    prefix_len.  gate [b, s, heads, d] multiplies by its sigmoid; scale defaults
+    to 1 / sqrt(head_dim); accumulate adds the probabilities to cache.weights
+    (`workspace`: a uint8 tensor of at least kv4_attention_workspace bytes, else
+    one is allocated on the current stream).  A sequence with a negative
+    cache_offset whose queries see nothing gives 0.  src/lib.rs:632-704.
+    """
+    _need(q, "q")
+    b, hk, _, d = cache.shape
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[1] % hk or q.shape[1] == 0:
+        raise ValueError(f"q must be [{b}, a multiple of {hk} heads, seq, {d}]")
+    h, s = q.shape[1], q.shape[2]
+    if out is None:
+        out = torch.empty((b, s, h, d), dtype=q.dtype, device=q.device)
+    else:
+        _need(out, "out")
+        if out.numel() != q.numel():
+            raise ValueError("out has the wrong size")
+    if gate is not None:
+        _need(gate, "gate")
+        if gate.numel() != q.numel():
+            raise ValueError("gate has the wrong size")
+    off, off_t = _offset(cache_offset, "cache_offset", b)
+    if accumulate and cache.weights is None:
+        raise ValueError("accumulate needs a cache with weights (kv4_cache(..., track=True))")
+    nbytes = 0
+    if accumulate:
+        nbytes = kv4_attention_workspace(cache, h, s)
+        if workspace is None:
+            # on the launch's stream, so that the allocator reuses it in that stream's order
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _need(workspace, "workspace", (torch.uint8,))
+        nbytes = workspace.numel()
+    else:
+        workspace = None
+    _launch("hrm_kv4_attention", (q, out, gate, cache.k_codes, off_t, workspace), stream, _ptr(q), cache._ref,
+            _ptr(gate), _ptr(out), h, s, off, _ptr(off_t), prefix_len, 1.0 / math.sqrt(d) if scale is None else scale,
+            int(accumulate), _ptr(workspace), nbytes)
+    return out
+
+
+def kv4_attention_workspace(cache: Kv4Cache, num_heads: int, seq_len: int, accumulate: bool = True) -> int:
+    """Bytes of workspace of such a kv4_attention call (0 without accumulate)."""
+    n = ctypes.c_int64(0)
+    call("hrm_kv4_attention_workspace", cache._ref, num_heads, seq_len, int(accumulate), ctypes.byref(n))
+    return n.value
+
+
+def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offset, out: Optional[Kv4Cache] = None,
+              new_lengths: Optional[torch.Tensor] = None, *, stream=None) -> torch.Tensor:
+    """Keeps the `budget` rows of largest weight of each kv head; returns the new lengths (int32 [b]).
+
+    lengths: the rows in use; rows whose position is at or past protect_from rank
+    above every weight.  In place, or into `out`, another tracked cache of at
+    least `budget` rows.  Kept rows below budget stay where they are, the others
+    fill the freed places in order.
+    """
+    to = cache if out is None else out
+    b, h, n, d = cache.shape
+    if cache.weights is None or cache.positions is None or to.weights is None or to.positions is None:
+        raise ValueError("kv4_evict needs caches with weights and positions (kv4_cache(..., track=True))")
+    if (to.shape[0], to.shape[1], to.shape[3]) != (b, h, d):
+        raise ValueError("out differs from the cache in batch, kv_heads or head_dim")
+    length, length_t = _offset(lengths, "lengths", b)
+    protect, protect_t = _offset(protect_from, "protect_from", b)
+    if new_lengths is None:
+        new_lengths = torch.empty(b, dtype=torch.int32, device=cache.k_codes.device)
+    _need(new_lengths, "new_lengths", (torch.int32,))
+    if new_lengths.numel() != b:
+        raise ValueError("new_lengths must have one value per sequence")
+    _launch("hrm_kv4_evict", (cache.k_codes, to.k_codes, length_t, protect_t, new_lengths), stream, cache._ref, to._ref,
+            length, _ptr(length_t), budget, protect, _ptr(protect_t), _ptr(new_lengths))
+    return new_lengths

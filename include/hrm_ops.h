@@ -41,7 +41,9 @@ enum hrm_status {
   HRM_ERR_ALIASING = 4,       /* buffers that must be distinct overlap           */
   HRM_ERR_TABLE_RANGE = 5,    /* position_offset + seq_len exceeds the rope table */
   HRM_ERR_DTYPE = 6,          /* unsupported element type                        */
-  HRM_ERR_SCRATCH_LIMIT = 7,  /* request larger than a fixed in-library scratch  */
+  HRM_ERR_SCRATCH_LIMIT = 7,  /* request larger than a fixed in-library scratch,
+                                 or a workspace smaller than the call needs    */
+  HRM_ERR_ALIGNMENT = 8,      /* a pointer is not aligned as its call requires   */
   HRM_ERR_CUDA = 1000         /* HRM_ERR_CUDA + cudaError_t of the failed launch  */
 };
 
@@ -253,6 +255,111 @@ int hrm_upload_to_bf16(const void* src, int src_dtype, void* dst, int64_t n, voi
  * streams, or from several host threads) race on it, so order them on one
  * stream.  Results equal hrm_upload_to_bf16's bit for bit.                  */
 int hrm_upload_to_bf16_static(const void* src, int src_dtype, void* dst, int64_t n, hrm_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* The 4-bit KV cache.
+ *
+ * The caller owns the buffers; the struct (host memory, read during the call
+ * only) names them.  Per (batch, kv head, row) of head_dim elements (64, 128,
+ * 192 or 256):
+ *   codes    head_dim / 2 bytes: byte i holds the code of element 2i in its low
+ *            nibble and of element 2i + 1 in its high one
+ *   scales   head_dim / 32 pairs of bf16 (S, Z), one per group of 32 elements
+ *   weights  fp32 accumulated attention weight     (optional: NULL)
+ *   positions int32 position of the row's token     (optional: NULL)
+ * and the cache stands for the bf16 values
+ *   value = bf16_rn(S * (1 + code / 16) + Z).
+ * The write calls choose, for a group's extremes lo and hi (fp32 operations),
+ *   S = bf16_rn((hi - lo) * (16/15)), 0 where hi - lo < 2^-100
+ *   Z = bf16_rn(lo - S)
+ *   code = clamp(rint((x - Z) * (16 / S) - 16), 0, 15), 0 where S == 0;
+ * a group that holds a NaN or an infinity, or whose S or Z overflows bf16,
+ * reads back as NaN.  All buffers are row-major [batch, kv_heads, cache_len, ...];
+ * codes and scales are 16-byte aligned (HRM_ERR_ALIGNMENT otherwise, also for
+ * the 16-bit tensors of these calls).  A row is 5 bits per element: 160 bytes
+ * for k and v of head_dim 128, against 512 in bf16.  No reference counterpart
+ * (its cache is bf16, src/kernels/kv_cache_update.cu:12-48).
+ *
+ * Offsets come as one host value or, where the array is not NULL, as one int32
+ * per sequence in device memory (the host value is then ignored), so that a
+ * captured graph can be replayed at the next position.  Host values are checked; values
+ * in device memory cannot be: rows outside [0, cache_len) are not written, and
+ * positions outside the rope table take in-kernel angles.                    */
+typedef struct hrm_kv4_cache {
+  void* k_codes;
+  void* k_scales;
+  void* v_codes;
+  void* v_scales;
+  float* weights;
+  int32_t* positions;
+  int64_t batch, kv_heads, cache_len, head_dim;
+} hrm_kv4_cache;
+
+/* Writes k and v ([batch, kv_heads, seq_len, head_dim] bf16) as rows
+ * cache_offset + s of the cache, s < seq_len; weights of those rows become 0
+ * and positions position_offset + s, where the cache has them.  The 4-bit
+ * counterpart of kv_cache_update (src/lib.rs:706-747).                       */
+int hrm_kv4_update(const hrm_kv4_cache* cache, const void* k, const void* v, int64_t seq_len, int64_t position_offset,
+                   const int32_t* position_offsets, int64_t cache_offset, const int32_t* cache_offsets,
+                   hrm_stream_t stream);
+
+/* hrm_split_gqkv_rope into a 4-bit cache (kv_heads = the heads of gqkv): gate_out
+ * and q_out as there, bit for bit; the rotated k, rounded to bf16, and the v of
+ * token s are written as hrm_kv4_update does.  k_out, v_out ([batch, heads, seq,
+ * head_dim], both or neither NULL) receive the values that the cache now stands
+ * for, so that a prefill attention over them agrees with later reads of the
+ * cache; they are written also for rows that fall outside the cache.          */
+int hrm_split_gqkv_rope_kv4(const void* gqkv, void* gate_out, void* q_out, void* k_out, void* v_out,
+                            const hrm_kv4_cache* cache, int64_t seq_len, int64_t position_offset,
+                            const int32_t* position_offsets, float theta, const float* rope_table,
+                            int64_t table_positions, int64_t cache_offset, const int32_t* cache_offsets,
+                            hrm_stream_t stream);
+
+/* Attention of q ([batch, num_heads, seq_len, head_dim] bf16) over the cache, whose
+ * rows [cache_offset, cache_offset + seq_len) already hold the queries' own tokens.
+ * Query s of sequence b sees the cache rows j < limit,
+ *   limit = min(max(cache_offset + s + 1, prefix_len), cache_offset + seq_len, cache_len)
+ * (prefix_len 0: causal; more: PrefixLM, as src/kernels/prefixlm_mask.cu:9-41):
+ *   p = softmax_j(softmax_scale * q . k_j),  out = sum_j p_j v_j
+ * in fp32 with one rounding at the end, times 1 / (1 + exp(-gate)) before that
+ * rounding where gate ([batch, seq_len, num_heads, head_dim] bf16) is not NULL.  out
+ * is [batch, seq_len, num_heads, head_dim], the layout of the gate and of the
+ * output projection.  num_heads is a multiple of kv_heads; query head h reads kv
+ * head h / (num_heads / kv_heads).  A query that sees no row (limit <= 0: a negative
+ * cache_offsets entry marks an idle sequence) gives 0.  Rows that a query does not
+ * see have no influence on it, whatever they hold.
+ * accumulate != 0 adds the probabilities to the cache's weights:
+ *   weights[b, kv head, j] += sum of p_j over the heads that share it and s,
+ * in an order that does not change from call to call.
+ * workspace: hrm_kv4_attention_workspace's bytes of device memory (0 without
+ * accumulate: NULL is fine), 16-byte aligned, free again once `stream` has
+ * passed this call.  Replaces mha and mha_decode (src/lib.rs:632-704,
+ * src/kernels/mha.cu:14-143, mha_decode.cu:15-140) for a 4-bit cache, with
+ * apply_attn_gate (src/lib.rs:920) as an optional epilogue.                    */
+int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gate, void* out, int64_t num_heads,
+                      int64_t seq_len, int64_t cache_offset, const int32_t* cache_offsets, int64_t prefix_len,
+                      float softmax_scale, int accumulate, void* workspace, int64_t workspace_bytes,
+                      hrm_stream_t stream);
+int hrm_kv4_attention_workspace(const hrm_kv4_cache* cache, int64_t num_heads, int64_t seq_len, int accumulate,
+                                int64_t* bytes);
+
+/* Eviction by accumulated attention weight.  Per (sequence, kv head), of the rows
+ * j < n (n = length, or lengths[b] clamped to [0, cache_len]) the min(n, budget)
+ * with the largest key stay; the key is +inf where positions[j] >= protect_from
+ * (the most recent tokens, say), else weights[j].  Of equal keys the lowest rows
+ * stay; a NaN weight ranks below every other.  Kept rows j < budget keep their
+ * place; the i-th kept row past them goes to the i-th freed place, with its codes,
+ * scales, weight and position.  Attention over earlier rows does not depend on
+ * their order, so the cache is then read with cache_offset = the new length.
+ * new_lengths[b] = min(n, budget); it must not overlap lengths.
+ * `out` may be the cache itself (in place: only the moved rows are written) or
+ * another cache of at least min(budget, n) rows, with no buffer shared.  Both need
+ * weights and positions.  Limit: 4 * min(budget, n - budget) + budget / 4 bytes
+ * (n the host length, or cache_len with `lengths`) may not pass 200 KB
+ * (HRM_ERR_SCRATCH_LIMIT).  No reference counterpart.                          */
+int hrm_kv4_evict(const hrm_kv4_cache* cache, const hrm_kv4_cache* out, int64_t length, const int32_t* lengths,
+                  int64_t budget, int64_t protect_from, const int32_t* protect_froms, int32_t* new_lengths,
+                  hrm_stream_t stream);
 
 /* Number of bounded device-side waits that ran out on the current device
  * since the library was loaded there (or since the last reset).  The
