@@ -78,17 +78,26 @@ int64_t attn_rows(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq_len) {
   return num_heads / c->kv_heads * seq_len;
 }
 
-int check_attention_shape(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq_len, int accumulate, int64_t* bytes) {
+// Bytes of workspace: the scores or the rows' sums that accumulate needs, then
+// the partial results of a split decode.
+struct AttnBytes {
+  int64_t tracked, parts;
+};
+
+int check_attention_shape(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq_len, int accumulate, AttnBytes* n) {
   if (num_heads <= 0 || seq_len < 0 || num_heads > INT32_MAX || num_heads % c->kv_heads != 0)
     return HRM_ERR_INVALID_SHAPE;
   if (seq_len > INT32_MAX) return HRM_ERR_SIZE_OVERFLOW;
   const int64_t rows = attn_rows(c, num_heads, seq_len), heads = c->batch * c->kv_heads;
   const int64_t all = mul_checked(heads, rows);
   if (all < 0 || all + 7 * heads > INT32_MAX || mul_checked(all, c->head_dim * 2) < 0) return HRM_ERR_SIZE_OVERFLOW;
-  if (mul_checked(heads, c->cache_len / 64 + 1) > INT32_MAX) return HRM_ERR_SIZE_OVERFLOW;
-  const int64_t scores = mul_checked(all, rows <= hrm::kDecodeRows ? c->cache_len : 1);
-  if (scores < 0 || mul_checked(scores, 4) < 0) return HRM_ERR_SIZE_OVERFLOW;
-  *bytes = accumulate ? scores * 4 : 0;
+  const int64_t tiles = c->cache_len / 64 + 1;  // of a head; (rows + 7) / 8 blocks of queries walk them
+  const int64_t walks = mul_checked(mul_checked(heads, (rows + 7) / 8), tiles);
+  if (walks < 0 || walks > INT32_MAX) return HRM_ERR_SIZE_OVERFLOW;
+  const int64_t tracked = mul_checked(mul_checked(all, rows <= hrm::kDecodeRows ? c->cache_len : 1), 4);
+  if (tracked < 0) return HRM_ERR_SIZE_OVERFLOW;
+  n->tracked = accumulate ? (tracked + 15) / 16 * 16 : 0;
+  n->parts = rows <= hrm::kChunkRows ? hrm::kv4_decode_workspace(rows, c->head_dim, c->cache_len) : 0;
   return HRM_OK;
 }
 
@@ -171,8 +180,11 @@ int hrm_kv4_attention_workspace(const hrm_kv4_cache* cache, int64_t num_heads, i
                                 int64_t* bytes) {
   if (!bytes) return HRM_ERR_NULL_POINTER;
   CacheBytes n;
-  const int e = check_cache_shape(cache, &n);
-  return e != HRM_OK ? e : check_attention_shape(cache, num_heads, seq_len, accumulate, bytes);
+  AttnBytes w{};
+  int e = check_cache_shape(cache, &n);
+  if (e == HRM_OK) e = check_attention_shape(cache, num_heads, seq_len, accumulate, &w);
+  if (e == HRM_OK) *bytes = w.tracked + w.parts;
+  return e;
 }
 
 int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gate, void* out, int64_t num_heads,
@@ -182,8 +194,8 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
   CacheBytes n;
   int e = check_cache_shape(cache, &n);
   if (e != HRM_OK) return e;
-  int64_t need = 0;
-  e = check_attention_shape(cache, num_heads, seq_len, accumulate, &need);
+  AttnBytes w{};
+  e = check_attention_shape(cache, num_heads, seq_len, accumulate, &w);
   if (e != HRM_OK) return e;
   e = check_places(cache, seq_len, 0, nullptr, cache_offset, cache_offsets);
   if (e != HRM_OK) return e;
@@ -196,8 +208,9 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
     if (accumulate && !cache->weights) return HRM_ERR_NULL_POINTER;
   } else {
     accumulate = 0;  // no row to add to
-    need = 0;
+    w.tracked = 0;
   }
+  const int64_t need = w.tracked + w.parts;
   if (need > 0 && !workspace) return HRM_ERR_NULL_POINTER;
   if (need > 0 && workspace_bytes < need) return HRM_ERR_SCRATCH_LIMIT;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(gate, 16) || (need > 0 && !aligned(workspace, 16)))
@@ -222,19 +235,20 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
   a.out = static_cast<uint16_t*>(out);
   a.c = view(cache);
   a.batch = cache->batch;
-  a.heads = num_heads;
-  a.kv_heads = cache->kv_heads;
-  a.group = num_heads / cache->kv_heads;
-  a.seq = seq_len;
+  a.heads = (int)num_heads;
+  a.kv_heads = (int)cache->kv_heads;
+  a.group = (int)(num_heads / cache->kv_heads);
+  a.seq = (int)seq_len;
   a.cache_offset = cache_offset;
   a.cache_offsets = cache_offsets;
   a.prefix_len = prefix_len;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  const int64_t rows = a.group * seq_len;
+  const int64_t rows = (int64_t)a.group * seq_len;
   if (accumulate) (rows <= hrm::kDecodeRows ? a.scores : a.lse) = static_cast<float*>(workspace);
   const int64_t longest = cache_offsets ? cache->cache_len : cache_offset + seq_len;
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.tracked);
   const cudaStream_t s = as_cuda(stream);
-  cudaError_t ce = rows <= hrm::kChunkRows ? hrm::launch_kv4_decode(a, cache->head_dim, longest, s)
+  cudaError_t ce = rows <= hrm::kChunkRows ? hrm::launch_kv4_decode(a, cache->head_dim, longest, parts, s)
                                            : hrm::launch_kv4_chunk(a, cache->head_dim, s);
   if (ce == cudaSuccess && a.lse != nullptr) ce = hrm::launch_kv4_weights(a, cache->head_dim, longest, s);
   return cuda_status(ce);

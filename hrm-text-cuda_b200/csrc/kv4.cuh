@@ -57,11 +57,17 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
 __device__ __forceinline__ uint32_t kv4_scale2(uint32_t sz) { return __byte_perm(sz, sz, 0x1010); }
 __device__ __forceinline__ uint32_t kv4_base2(uint32_t sz) { return __byte_perm(sz, sz, 0x3232); }
 
-// 1 + n/16 of nibbles P and P + 4 of w, as a packed bf16 pair.
+// 1 + n/16 of nibbles P and P + 4 of w, as a packed bf16 pair: one shift and one
+// three-input and-or (written out: the compiler made two instructions of it).
+// Extracting nibbles 0 and 1 without a shift, by packed fmas that scale the masked
+// bits, measured slower: the fma's pipe is no less busy, and denormal operands
+// (bits 4-7 alone) cost it several times a normal one.
 template <int P>
 __device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
   const uint32_t x = P == 0 ? w << 3 : w >> (P == 0 ? 0 : 4 * P - 3);
-  return (x & 0x00780078u) | 0x3f803f80u;
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(0x00780078u), "r"(0x3f803f80u));
+  return r;
 }
 
 // Quantises 8 elements per lane; the 4 lanes of an aligned quad hold one group

@@ -313,9 +313,9 @@ __global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const AttnArgs a,
 
 template <int D>
 cudaError_t launch_chunk(const AttnArgs& a, cudaStream_t s) {
-  const int64_t tiles = (a.group * a.seq + kM - 1) / kM, grid = a.batch * a.kv_heads * tiles;
+  const int64_t tiles = ((int64_t)a.group * a.seq + kM - 1) / kM, grid = a.batch * a.kv_heads * tiles;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = allow_shared(kv4_chunk_kernel<D>, Chunk<D>::kSmem);
+  const cudaError_t e = allow_shared<kv4_chunk_kernel<D>>(Chunk<D>::kSmem);
   if (e != cudaSuccess) return e;
   return launch_kernel(kv4_chunk_kernel<D>, grid, kThreads, Chunk<D>::kSmem, s, a, tiles);
 }
@@ -324,7 +324,7 @@ template <int D>
 cudaError_t launch_weights(const AttnArgs& a, int64_t longest, cudaStream_t s) {
   const int64_t tiles = (longest + kN - 1) / kN, grid = a.batch * a.kv_heads * tiles;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = allow_shared(kv4_weights_kernel<D>, Chunk<D>::kV);
+  const cudaError_t e = allow_shared<kv4_weights_kernel<D>>(Chunk<D>::kV);
   if (e != cudaSuccess) return e;
   return launch_kernel(kv4_weights_kernel<D>, grid, kThreads, Chunk<D>::kV, s, a, tiles);
 }

@@ -63,6 +63,7 @@ __device__ __forceinline__ int cta_sum(int x, int* buf) {
 // Words of shared memory: the moving rows in order, then a bit per place that
 // keeps its row and, per 32 places, how many are freed before them.
 inline int64_t evict_moves(int64_t n, int64_t budget) { return n <= budget ? 0 : (n - budget < budget ? n - budget : budget); }
+constexpr size_t kSharedMost = 200 * 1024;
 inline size_t evict_shared(int64_t n, int64_t budget) {
   return 4 * (size_t)(evict_moves(n, budget) + 2 * ((budget + 31) / 32));
 }
@@ -267,7 +268,8 @@ __global__ void __launch_bounds__(W * 32) kv4_evict_kernel(const EvictArgs a, co
 template <int W, int K>
 cudaError_t launch(const EvictArgs& a, int64_t batch, int64_t n, int shares, cudaStream_t s) {
   const size_t smem = evict_shared(n, a.budget);
-  const cudaError_t e = allow_shared(kv4_evict_kernel<W, K>, smem);
+  // the size varies from call to call: allow the largest that kv4_evict_fits lets through
+  const cudaError_t e = smem <= 48 * 1024 ? cudaSuccess : allow_shared<kv4_evict_kernel<W, K>>(kSharedMost);
   if (e != cudaSuccess) return e;
   const int64_t grid = batch * a.kv_heads * shares;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -276,7 +278,7 @@ cudaError_t launch(const EvictArgs& a, int64_t batch, int64_t n, int shares, cud
 
 }  // namespace
 
-bool kv4_evict_fits(int64_t n, int64_t budget) { return evict_shared(n, budget) <= 200 * 1024; }
+bool kv4_evict_fits(int64_t n, int64_t budget) { return evict_shared(n, budget) <= kSharedMost; }
 
 cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_place, int64_t batch, int64_t kv_heads,
                              int64_t head_dim, int64_t length, const int* lengths, int64_t budget,

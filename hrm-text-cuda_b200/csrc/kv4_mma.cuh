@@ -13,12 +13,15 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2^x, within 2 ulp; 0
 // D = A (16x16, row) * B (16x8, col) + D, bf16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// cp.async of BYTES (4, 8 or 16) global -> shared; zeros where !valid (src is not read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+// cp.async of BYTES (8 or 16) global -> shared; zeros where !valid (src is not read then).
 template <int BYTES>
 __device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? BYTES : 0;
@@ -45,7 +48,8 @@ struct AttnArgs {
   const uint16_t* gate;  // [batch, seq, heads, D] bf16, or null
   uint16_t* out;         // [batch, seq, heads, D] bf16
   Kv4View c;
-  int64_t batch, heads, kv_heads, group, seq;
+  int64_t batch;
+  int heads, kv_heads, group, seq;  // group * seq * batch * kv_heads fits in 31 bits
   int64_t cache_offset;
   const int* cache_offsets;  // per sequence, or null
   int64_t prefix_len;
@@ -55,7 +59,7 @@ struct AttnArgs {
 };
 
 // Cache rows that query s of sequence b sees: [0, limit).
-__device__ __forceinline__ int visible_rows(const AttnArgs& a, int64_t b, int64_t s) {
+__device__ __forceinline__ int visible_rows(const AttnArgs& a, int b, int s) {
   const int64_t off = a.cache_offsets ? a.cache_offsets[b] : a.cache_offset;
   int64_t lim = off + s + 1;
   if (lim < a.prefix_len) lim = a.prefix_len;

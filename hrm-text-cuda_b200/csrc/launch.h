@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace hrm {
 
 // SM count of the current device, queried once per device and cached.
@@ -70,12 +72,21 @@ inline cudaError_t launch_cluster(void (*k)(KArgs...), int64_t grid, int block, 
   return cudaLaunchKernelEx(&cfg, k, static_cast<Args&&>(args)...);
 }
 
-// Lets kernel k be launched with `bytes` of dynamic shared memory on the current
-// device (needed above 48 KB).
-template <typename... KArgs>
-inline cudaError_t allow_shared(void (*k)(KArgs...), size_t bytes) {
-  return bytes <= 48 * 1024 ? cudaSuccess
-                            : cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+// Lets kernel K be launched with `bytes` of dynamic shared memory on the current
+// device (needed above 48 KB).  The driver call is made once per kernel and device:
+// a call costs the host about as much as a launch's own bookkeeping.
+template <auto K>
+inline cudaError_t allow_shared(size_t bytes) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 cudaError_t launch_additive_inject(const void* a, const void* b, void* out, int64_t n, cudaStream_t s);
@@ -115,8 +126,10 @@ cudaError_t launch_split_rope_kv4(const void* gqkv, void* gate, void* q, void* k
 cudaError_t launch_kv4_update(const void* k, const void* v, const Kv4View& c, int64_t batch, int64_t heads,
                               int64_t seq, int64_t head_dim, int64_t position_offset, const int* position_offsets,
                               int64_t cache_offset, const int* cache_offsets, cudaStream_t s);
-// `longest`: no sequence has more cache rows than this.
-cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s);
+// `longest`: no sequence has more cache rows than this; `parts`: kv4_decode_workspace
+// bytes for the same sizes.
+int64_t kv4_decode_workspace(int64_t rows, int64_t head_dim, int64_t longest);
+cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s);
 cudaError_t launch_kv4_chunk(const AttnArgs& a, int64_t head_dim, cudaStream_t s);
 cudaError_t launch_kv4_weights(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s);
 // Whether the selection of `budget` out of at most n rows fits its shared memory.

@@ -21,13 +21,44 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import Kv4CacheStruct, call
-from .ops import _launch, _need, _ptr
+from ._lib import HRM_OK, LIB, Kv4CacheStruct, check
+from .ops import _need
 
 GROUP = 32  # elements per (scale, base) pair
 HEAD_DIMS = (64, 128, 192, 256)
 
 Offset = Union[int, torch.Tensor]
+
+# The handle of a device's current stream, without the Stream object around it (a
+# decode step makes one such call per layer and operator).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(name: str, device: torch.device, tensors, stream: Optional[torch.cuda.Stream], *args) -> None:
+    """ops._launch for calls of a few microseconds: the same checks (every tensor and
+    an explicit stream on `device`, which is current during the call), on plain
+    integers."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: tensors on {device} and {t.device}; every argument must be on one device")
+    if stream is None:
+        handle = _raw_stream(device.index)
+    elif stream.device != device:
+        raise ValueError(f"{name}: stream on {stream.device} but tensors on {device}")
+    else:
+        handle = stream.cuda_stream
+    if torch.cuda.current_device() == device.index:
+        status = getattr(LIB, name)(*args, handle)
+    else:
+        with torch.cuda.device(device):
+            status = getattr(LIB, name)(*args, handle)
+    if status != HRM_OK:
+        check(name, status)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 @dataclass
@@ -73,6 +104,8 @@ class Kv4Cache:
                for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.weights, self.positions)]
         self._struct = Kv4CacheStruct(*ptr, b, h, n, 2 * half)
         self._ref = ctypes.pointer(self._struct)
+        self.device = self.k_codes.device
+        self._workspaces = {}  # bytes by (heads, seq, accumulate)
 
 
 def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, device=None, track: bool = False) -> Kv4Cache:
@@ -112,7 +145,7 @@ def kv4_update(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, position_offse
         raise ValueError(f"k and v must both be [{b}, {h}, seq, {d}]")
     pos, pos_t = _offset(position_offset, "position_offset", b)
     off, off_t = _offset(cache_offset, "cache_offset", b)
-    _launch("hrm_kv4_update", (k, v, cache.k_codes, pos_t, off_t), stream, cache._ref, _ptr(k), _ptr(v), k.shape[2], pos,
+    _launch("hrm_kv4_update", cache.device, (k, v, pos_t, off_t), stream, cache._ref, _ptr(k), _ptr(v), k.shape[2], pos,
             _ptr(pos_t), off, _ptr(off_t))
     return cache
 
@@ -131,9 +164,9 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
     s = gqkv.shape[1]
     if out is None:
-        new = lambda *shape: torch.empty(shape, dtype=gqkv.dtype, device=gqkv.device)  # noqa: E731
-        out = (new(b, s, h, d), new(b, h, s, d), new(b, h, s, d) if keep_kv else None,
-               new(b, h, s, d) if keep_kv else None)
+        new = gqkv.new_empty
+        kv = (b, h, s, d)
+        out = (new((b, s, h, d)), new(kv), new(kv) if keep_kv else None, new(kv) if keep_kv else None)
     for t, n in zip(out, ("gate", "q", "k", "v")):
         if t is None and n in ("k", "v"):
             continue
@@ -148,7 +181,7 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         positions = table.shape[0]
     pos, pos_t = _offset(position_offset, "position_offset", b)
     off, off_t = _offset(cache_offset, "cache_offset", b)
-    _launch("hrm_split_gqkv_rope_kv4", (gqkv, *out, cache.k_codes, table, pos_t, off_t), stream, _ptr(gqkv),
+    _launch("hrm_split_gqkv_rope_kv4", cache.device, (gqkv, *out, table, pos_t, off_t), stream, _ptr(gqkv),
             *(_ptr(t) for t in out), cache._ref, s, pos, _ptr(pos_t), theta, _ptr(table), positions, off, _ptr(off_t))
     return tuple(out)
 
@@ -173,7 +206,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
         raise ValueError(f"q must be [{b}, a multiple of {hk} heads, seq, {d}]")
     h, s = q.shape[1], q.shape[2]
     if out is None:
-        out = torch.empty((b, s, h, d), dtype=q.dtype, device=q.device)
+        out = q.new_empty((b, s, h, d))
     else:
         _need(out, "out")
         if out.numel() != q.numel():
@@ -185,28 +218,33 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
     off, off_t = _offset(cache_offset, "cache_offset", b)
     if accumulate and cache.weights is None:
         raise ValueError("accumulate needs a cache with weights (kv4_cache(..., track=True))")
-    nbytes = 0
-    if accumulate:
-        nbytes = kv4_attention_workspace(cache, h, s)
-        if workspace is None:
-            # on the launch's stream, so that the allocator reuses it in that stream's order
+    nbytes = kv4_attention_workspace(cache, h, s, accumulate)
+    if nbytes and workspace is None:
+        if stream is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        else:  # on the launch's stream, so that the allocator reuses it in that stream's order
             with torch.cuda.stream(stream):
                 workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    elif workspace is not None:
         _need(workspace, "workspace", (torch.uint8,))
         nbytes = workspace.numel()
-    else:
-        workspace = None
-    _launch("hrm_kv4_attention", (q, out, gate, cache.k_codes, off_t, workspace), stream, _ptr(q), cache._ref,
+    _launch("hrm_kv4_attention", cache.device, (q, out, gate, off_t, workspace), stream, _ptr(q), cache._ref,
             _ptr(gate), _ptr(out), h, s, off, _ptr(off_t), prefix_len, 1.0 / math.sqrt(d) if scale is None else scale,
             int(accumulate), _ptr(workspace), nbytes)
     return out
 
 
 def kv4_attention_workspace(cache: Kv4Cache, num_heads: int, seq_len: int, accumulate: bool = True) -> int:
-    """Bytes of workspace of such a kv4_attention call (0 without accumulate)."""
-    n = ctypes.c_int64(0)
-    call("hrm_kv4_attention_workspace", cache._ref, num_heads, seq_len, int(accumulate), ctypes.byref(n))
-    return n.value
+    """Bytes of workspace of such a kv4_attention call (may be 0)."""
+    key = (num_heads, seq_len, accumulate)
+    n = cache._workspaces.get(key)
+    if n is None:
+        size = ctypes.c_int64(0)
+        with torch.cuda.device(cache.device):
+            check("hrm_kv4_attention_workspace", LIB.hrm_kv4_attention_workspace(cache._ref, num_heads, seq_len,
+                                                                                 int(accumulate), ctypes.byref(size)))
+        n = cache._workspaces[key] = size.value
+    return n
 
 
 def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offset, out: Optional[Kv4Cache] = None,
@@ -227,10 +265,10 @@ def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offse
     length, length_t = _offset(lengths, "lengths", b)
     protect, protect_t = _offset(protect_from, "protect_from", b)
     if new_lengths is None:
-        new_lengths = torch.empty(b, dtype=torch.int32, device=cache.k_codes.device)
+        new_lengths = torch.empty(b, dtype=torch.int32, device=cache.device)
     _need(new_lengths, "new_lengths", (torch.int32,))
     if new_lengths.numel() != b:
         raise ValueError("new_lengths must have one value per sequence")
-    _launch("hrm_kv4_evict", (cache.k_codes, to.k_codes, length_t, protect_t, new_lengths), stream, cache._ref, to._ref,
+    _launch("hrm_kv4_evict", cache.device, (to.k_codes, length_t, protect_t, new_lengths), stream, cache._ref, to._ref,
             length, _ptr(length_t), budget, protect, _ptr(protect_t), _ptr(new_lengths))
     return new_lengths

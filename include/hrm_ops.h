@@ -331,9 +331,9 @@ int hrm_split_gqkv_rope_kv4(const void* gqkv, void* gate_out, void* q_out, void*
  * accumulate != 0 adds the probabilities to the cache's weights:
  *   weights[b, kv head, j] += sum of p_j over the heads that share it and s,
  * in an order that does not change from call to call.
- * workspace: hrm_kv4_attention_workspace's bytes of device memory (0 without
- * accumulate: NULL is fine), 16-byte aligned, free again once `stream` has
- * passed this call.  Replaces mha and mha_decode (src/lib.rs:632-704,
+ * workspace: hrm_kv4_attention_workspace's bytes of device memory (asked for with
+ * the launch's device current; it may be 0, then NULL is fine), 16-byte aligned,
+ * free again once `stream` has passed this call.  Replaces mha and mha_decode (src/lib.rs:632-704,
  * src/kernels/mha.cu:14-143, mha_decode.cu:15-140) for a 4-bit cache, with
  * apply_attn_gate (src/lib.rs:920) as an optional epilogue.                    */
 int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gate, void* out, int64_t num_heads,

@@ -423,3 +423,53 @@ def test_evict_all_rows_protected_or_none(cuda):
     check_evict(c, 700, 128, 0, out)
     check_evict(c, 700, 128, 10**7, out)
     check_evict(c, 100, 128, 0, out)
+
+
+# ----------------------------------------------- long caches: shares of all items
+@pytest.mark.parametrize("b,hk,group,s,n,d,ragged", [(1, 1, 1, 1, 4097, 64, False), (1, 3, 1, 1, 20000, 128, False),
+                                                     (5, 2, 1, 1, 9000, 128, True), (70, 1, 1, 1, 4200, 64, True),
+                                                     (3, 1, 4, 2, 6000, 256, True), (2, 1, 2, 9, 5000, 128, True),
+                                                     (40, 16, 1, 1, 4500, 64, True), (2, 1, 1, 3, 4300, 192, False)])
+def test_attention_long_caches(cuda, b, hk, group, s, n, d, ragged):
+    """The rows of all items laid end to end and cut: against the 64-bit form, with weights."""
+    c = filled(b, hk, n, d, 7 * n)
+    q, gate = rand((b, hk * group, s, d), 1), rand((b, s, hk * group, d), 2)
+    if ragged:  # full, empty and short sequences among them
+        off = torch.tensor([(n - s) if i % 4 == 0 else (-s - 1 if i % 4 == 1 else (n - s) * i // (4 * b))
+                            for i in range(b)], dtype=torch.int32, device="cuda")
+    else:
+        off = n - s
+    if b * hk * group * s <= 40:
+        run_attention(c, q, off, gate=gate, accumulate=True)
+        return
+    # many rows: vectorised over heads
+    k, v = ref.values(c.k_codes, c.k_scales), ref.values(c.v_codes, c.v_scales)
+    w0 = c.weights.double()
+    got = ops.kv4_attention(q, c, off, gate=gate, accumulate=True)
+    lim = ref.limits(off, s, 0, n).cuda()
+    x = torch.einsum("bhsd,bhld->bhsl", q.double(), k) * d**-0.5
+    seen = torch.arange(n, device="cuda") < lim[:, None, :, None]
+    p = torch.softmax(x.masked_fill(~seen, -float("inf")), -1).nan_to_num(0.0)
+    sig = torch.sigmoid(gate.double())
+    want = torch.einsum("bhsl,bhld->bshd", p, v) * sig
+    spread = torch.einsum("bhsl,bhld->bshd", p, v.abs()) * sig
+    e = (d + 8) * 2.0**-23 * float((q.double().abs().amax() * k.abs().sum(-1).amax())) * d**-0.5
+    rel = 2 * e + (n + 64) * 2.0**-23 + 2.0**-20 + 2.0**-18 + 2.0**-16
+    assert bool(((got.double() - want).abs() <= U * want.abs() + rel * spread + 1e-37).all())
+    err, w = (c.weights.double() - w0 - p.sum(2)).abs(), p.sum(2)
+    assert bool((err <= rel * w + 2.0**-21 * (w0 + w)).all())
+
+
+def test_long_caches_nan_rows_and_lse_order(cuda):
+    """Not-seen NaN tokens at the end of a cut item; the same result from call to call."""
+    n, d, s = 9000, 128, 4
+    c = filled(1, 2, n, d, 33)
+    q = rand((1, 2, s, d), 34)
+    clean = ops.kv4_attention(q, c, n - s)
+    c.v_scales[:, :, n - 1, 1, 0] = float("nan")
+    for _ in range(3):
+        got = ops.kv4_attention(q, c, n - s)
+        same(got[:, :-1], clean[:, :-1])
+        nan = torch.isnan(got[0, -1])
+        want = torch.zeros_like(nan); want[:, 32:64] = True
+        assert torch.equal(nan, want)
