@@ -309,7 +309,11 @@ int hrm_upload_to_bf16(const void* src, int src_dtype, void* dst, int64_t n, voi
 
 int hrm_wait_timeouts(unsigned int* count, int reset) {
   if (!count) return HRM_ERR_NULL_POINTER;
-  return cuda_status(hrm::rownorm_wait_timeouts(count, reset != 0));
+  unsigned int more = 0;
+  cudaError_t e = hrm::rownorm_wait_timeouts(count, reset != 0);
+  if (e == cudaSuccess) e = hrm::kv4_prefill_wait_timeouts(&more, reset != 0);
+  *count += more;
+  return cuda_status(e);
 }
 
 }  // extern "C"

@@ -332,12 +332,7 @@ cudaError_t launch_weights(const AttnArgs& a, int64_t longest, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_kv4_chunk(const AttnArgs& a, int64_t head_dim, cudaStream_t s) {
-  switch (head_dim) {
-    case 64: return launch_chunk<64>(a, s);
-    case 128: return launch_chunk<128>(a, s);
-    case 192: return launch_chunk<192>(a, s);
-    default: return launch_chunk<256>(a, s);
-  }
+  return head_dim == 192 ? launch_chunk<192>(a, s) : launch_chunk<256>(a, s);
 }
 
 cudaError_t launch_kv4_weights(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s) {
