@@ -98,8 +98,7 @@ int check_attention_shape(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq
   if (tracked < 0) return HRM_ERR_SIZE_OVERFLOW;
   n->tracked = accumulate ? (tracked + 15) / 16 * 16 : 0;
   n->parts = rows <= hrm::kChunkRows ? hrm::kv4_decode_workspace(rows, c->head_dim, c->cache_len)
-             : c->head_dim <= 128    ? hrm::kv4_prefill_workspace(heads, rows, c->head_dim)
-                                     : 0;
+                                       : hrm::kv4_prefill_workspace(heads, rows, c->head_dim);
   return HRM_OK;
 }
 
@@ -251,8 +250,7 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.tracked);
   const cudaStream_t s = as_cuda(stream);
   cudaError_t ce = rows <= hrm::kChunkRows ? hrm::launch_kv4_decode(a, cache->head_dim, longest, parts, s)
-                   : cache->head_dim <= 128 ? hrm::launch_kv4_prefill(a, cache->head_dim, longest, parts, s)
-                                            : hrm::launch_kv4_chunk(a, cache->head_dim, s);
+                                           : hrm::launch_kv4_prefill(a, cache->head_dim, longest, parts, s);
   if (ce == cudaSuccess && a.lse != nullptr) ce = hrm::launch_kv4_weights(a, cache->head_dim, longest, s);
   return cuda_status(ce);
 }

@@ -357,8 +357,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& x, int t0,
   // words' 8 elements in the order in which kv4_pair yields them
   uint32_t q[T::kLaneWords][4];
   {
-    const Place p = place_of(a, x, !ONE && g < x.nrows ? g : 0);
-    const uint4* src = a.q + (((int64_t)x.b * a.heads + p.h) * a.seq + p.s) * (D / 8);
+    // (the query rows of a kv head lie one after another)
+    const int64_t row = ((int64_t)x.b * a.heads + x.hk * a.group) * a.seq + x.row0 + (!ONE && g < x.nrows ? g : 0);
+    const uint4* src = a.q + row * (D / 8);
 #pragma unroll
     for (int i = 0; i < T::kLaneWords; ++i) {
       uint4 v = ld_keep(src + k_word<D>(i, t));

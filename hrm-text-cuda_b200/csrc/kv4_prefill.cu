@@ -1,18 +1,22 @@
-// Attention of many query rows over the 4-bit cache on tcgen05, head_dim 64 and
-// 128: prompts and further turns of a chat.
+// Attention of many query rows over the 4-bit cache on tcgen05 (prompts and further
+// turns of a chat), and the pass that adds the probabilities of many query rows to
+// the cache rows' weights.
 //
 // A CTA owns NQ x 128 query rows of one kv head and walks its share of the cache in
-// tiles of 128 rows.  Three kinds of warps work at once, handing tiles over by
+// tiles of N rows: NQ = 2 and N = 128 up to head_dim 128, 1 and 64 above, where the
+// operands of two stages fill the shared memory.  Two kinds of warps work at once, handing tiles over by
 // mbarriers:
 //   * 4 warps dequantise: codes and scales from global memory (the next tile's are
 //     loaded while this one is converted), bf16 operands to shared memory, two
 //     stages.  k is stored as it lies, [row][element]; v transposed, [element][row],
 //     two cache rows' half words put together before the conversion, so that both
 //     operands are K-major.
-//   * one thread issues the products: S = Q K^T (128 x 128, accumulated in tensor
-//     memory) and O += P V with P read from tensor memory, where it replaces S.
-//     With NQ = 2 the products of one query tile run while the other's softmax does.
-//   * 4 warps per query tile do the softmax, a thread per row: no shuffles.  O is
+//   * 4 warps per query tile do the softmax, a thread per row, the row in registers:
+//     no shuffles.  One of their threads issues the tile's products: S = Q K^T (128 x N,
+//     accumulated in tensor memory) and O += P V with P read from tensor memory, where
+//     it replaces S.  With NQ = 2 the products of one query tile run while the other's
+//     softmax does.  (A warp of its own for the products would make 13 warps, and 4 on
+//     one scheduler leave a thread 128 registers: too few for a row of 128.)  O is
 //     rescaled only when a row's maximum has grown by more than 8 (in log2 units)
 //     since its last rescale: until then probabilities may be as large as 2^8,
 //     which neither the bf16 P nor the fp32 sums mind.
@@ -32,19 +36,23 @@ namespace hrm {
 namespace {
 
 constexpr int kM = 128;  // query rows of a tile
-constexpr int kN = 128;  // cache rows of a tile
 constexpr float kSlack = 8.0f;
+
+template <int D>
+constexpr int tile_rows() { return D <= 128 ? 128 : 64; }
+constexpr uint32_t tmem_columns(int used) { return used <= 128 ? 128 : used <= 256 ? 256 : 512; }
 
 template <int D, int NQ>
 struct Pre {
+  static constexpr int kN = tile_rows<D>();  // cache rows of a tile
   static constexpr int kGroups = D / kKv4Group;
   static constexpr int kSoftmax = NQ * 128, kFill = 128;
-  static constexpr int kThreads = kSoftmax + kFill + 32;
+  static constexpr int kThreads = kSoftmax + kFill;
   static constexpr int kQ = 0, kQBytes = kM * D * 2;              // per query tile
   static constexpr int kK = NQ * kQBytes, kKBytes = kN * D * 2;   // per stage
   static constexpr int kV = kK + 2 * kKBytes, kVBytes = D * kN * 2;
   static constexpr int kSmem = kV + 2 * kVBytes + 1024;  // + alignment of the panels
-  static constexpr uint32_t kColumns = NQ == 2 ? 512 : 256;  // S of each tile, then O of each
+  static constexpr uint32_t kColumns = tmem_columns(NQ * (kN + D));  // S of each tile, then O of each
 };
 
 // Barriers, in order.
@@ -52,9 +60,9 @@ enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10
 
 struct PrefillSplit {
   int count;     // CTAs per item (kv head x block of query rows)
-  float* parts;  // per (item, split): NQ * 128 rows of D sums, then the maxima, the sums and the masks
+  float* parts;  // per (item, split), [D][rows] sums, then the rows' maxima, sums and masks; rows = NQ * 128
 };
-__host__ __device__ inline int64_t prefill_part(int nq, int64_t head_dim) { return nq * kM * (head_dim + 4); }
+__host__ __device__ inline int64_t prefill_part(int nq, int64_t head_dim) { return nq * kM * (head_dim + 3); }
 
 // Element x of a row's order of elements in shared memory: within 8, kv4_pair's order.
 __device__ __forceinline__ uint4 paired_order(const uint4& v) {
@@ -62,21 +70,26 @@ __device__ __forceinline__ uint4 paired_order(const uint4& v) {
                     __byte_perm(v.y, v.w, 0x7632));
 }
 
-// A filling thread's share of a tile: D / 32 pieces (16 bytes of codes, one group) of
-// k, and one piece of 4 adjacent rows of v (D = 64: half the threads).  The lanes'
-// rows are such that a warp's loads fill whole sectors and its stores fall into
-// different banks.
-template <int D>
+// A filling thread's share of a tile of N rows: pieces (16 bytes of codes, one group)
+// of k, and one piece of 4 adjacent rows of v (where there are fewer of those than
+// threads, some threads have none).  The lanes' rows are such that a warp's loads
+// fill whole sectors and its stores fall into different banks: 16 lanes have 16
+// rows (or quads of rows) of one piece, the other 16 the next piece.
+template <int D, int N>
 struct Codes {
-  static constexpr int kK = D / 32;
+  static constexpr int kPieces = D / 32;  // per row
+  static constexpr int kK = N * kPieces / 128;
   uint4 k[kK], v[4];
   uint32_t ks[kK], vs[4];
 
-  __device__ __forceinline__ static int k_row(int i, int t) { return (t >> 5) * 32 + i / (D / 64) * 16 + (t & 15); }
-  __device__ __forceinline__ static int k_piece(int i, int t) { return i % (D / 64) * 2 + ((t >> 4) & 1); }
-  __device__ __forceinline__ static bool v_works(int t) { return D == 128 || t < 64; }
-  __device__ __forceinline__ static int v_quad(int t) { return ((t >> 5) & 1) * 16 + (t & 15); }
-  __device__ __forceinline__ static int v_piece(int t) { return (t >> 6) * 2 + ((t >> 4) & 1); }
+  // of the half warp number h, in order: first the pieces, then the rows
+  __device__ __forceinline__ static int piece(int h) { return (h & 1) + 2 * ((h >> 1) % (kPieces / 2)); }
+  __device__ __forceinline__ static int sixteen(int h) { return (h >> 1) / (kPieces / 2); }
+  __device__ __forceinline__ static int k_row(int i, int t) { return sixteen(8 * i + (t >> 4)) * 16 + (t & 15); }
+  __device__ __forceinline__ static int k_piece(int i, int t) { return piece(8 * i + (t >> 4)); }
+  __device__ __forceinline__ static bool v_works(int t) { return (t >> 4) < N / 64 * kPieces; }
+  __device__ __forceinline__ static int v_quad(int t) { return sixteen(t >> 4) * 16 + (t & 15); }
+  __device__ __forceinline__ static int v_piece(int t) { return piece(t >> 4); }
 
   // codes, scales: at the head's first row
   __device__ __forceinline__ void fetch_k(const uint8_t* codes, const uint32_t* scales, int first, int limit, int t) {
@@ -106,8 +119,8 @@ struct Codes {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t x = vget(k[i], w);
-        const int piece = 4 * p + w;
-        *reinterpret_cast<uint4*>(dst + (piece / 8) * (kN * 128) + panel_piece(row, piece % 8)) =
+        const int c = 4 * p + w;  // 16-byte piece of the row in bf16
+        *reinterpret_cast<uint4*>(dst + (c / 8) * (N * 128) + panel_piece(row, c % 8)) =
             make_uint4(fma_bf16x2(kv4_pair<0>(x), s2, z2), fma_bf16x2(kv4_pair<1>(x), s2, z2),
                        fma_bf16x2(kv4_pair<2>(x), s2, z2), fma_bf16x2(kv4_pair<3>(x), s2, z2));
       }
@@ -115,7 +128,7 @@ struct Codes {
   }
   // bf16 v to the panels at dst, [element][row].  With `flags`, groups that are not
   // finite are stored as zeros and marked there.
-  __device__ __forceinline__ void store_v(uint8_t* dst, int t, uint8_t (*flags)[4]) {
+  __device__ __forceinline__ void store_v(uint8_t* dst, int t, uint8_t (*flags)[8]) {
     if (!v_works(t)) return;
     const int q = v_quad(t), p = v_piece(t);
     if (flags != nullptr) {
@@ -152,24 +165,28 @@ template <int D, int NQ>
 __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     kv4_prefill_kernel(const AttnArgs a, const PrefillSplit split, const int blocks_q) {
   using T = Pre<D, NQ>;
+  constexpr int kN = T::kN;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kBars];
   __shared__ uint32_t s_tmem;
   __shared__ int s_limit[NQ * kM];
-  __shared__ __align__(16) uint8_t s_bad[2][kN][4];  // per stage and cache row: groups of v that are not finite
+  __shared__ __align__(16) uint8_t s_bad[2][kN][8];  // per stage and cache row: groups of v that are not finite
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
   auto bar = [&](int i) -> uint32_t { return bar0 + 8 * i; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kMmaWarp = (T::kSoftmax + T::kFill) / 32;
   grid_dependency_begin();
 
   const unsigned rows = a.group * a.seq;
   const unsigned item = blockIdx.x / split.count;
   const int rank = (int)(blockIdx.x - item * split.count);
-  const int bh = (int)(item / blocks_q), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
-  // the last rows first: under a causal mask they have the most tiles
-  const unsigned row0 = (blocks_q - 1 - (item - bh * blocks_q)) * (NQ * kM);
+  // all heads' last rows first: under a causal mask they have the most tiles
+  const unsigned heads_all = (unsigned)(a.batch * a.kv_heads), back = item / heads_all;
+  const int bh = (int)(item - back * heads_all), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
+  const unsigned row0 = (blocks_q - 1 - back) * (NQ * kM);
+  // query row r of the kv head is query r % seq of its head r / seq: they lie one after
+  // another (worked out where it is needed: the softmax has no register to spare)
+  auto q_row0 = [&]() -> int64_t { return ((int64_t)b * a.heads + hk * a.group) * a.seq; };
 
   // ---- set-up: limits, queries, barriers, tensor memory
   for (int r = tid; r < NQ * kM; r += T::kThreads) {
@@ -179,27 +196,34 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   {
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;  // the softmax takes |scale|
     const uint32_t keep = a.scale_log2 == 0.0f ? 0u : 0xffffffffu;  // scale 0: all scores 0
-    for (int i = tid; i < NQ * kM * (D / 8); i += T::kThreads) {
-      const int r = i / (D / 8), p = i % (D / 8);
-      const unsigned row = row0 + r;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows) {
-        const unsigned g = row / a.seq, s = row - g * a.seq;
-        v = ld_keep(a.q + (((int64_t)b * a.heads + hk * a.group + g) * a.seq + s) * (D / 8) + p);
+    constexpr int kAhead = 8;  // pieces in flight at once per thread
+    const uint4* src = a.q + (q_row0() + row0) * (D / 8);
+    for (int i0 = tid; i0 < NQ * kM * (D / 8); i0 += kAhead * T::kThreads) {
+      uint4 v[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * T::kThreads, r = i / (D / 8);
+        v[x] = make_uint4(0, 0, 0, 0);
+        if (i < NQ * kM * (D / 8) && row0 + r < rows) v[x] = ld_keep(src + i);
       }
-      v = paired_order(v);
-      v = make_uint4((v.x ^ flip) & keep, (v.y ^ flip) & keep, (v.z ^ flip) & keep, (v.w ^ flip) & keep);
-      *reinterpret_cast<uint4*>(smem + (r / kM) * T::kQBytes + (p / 8) * (kM * 128) + panel_piece(r % kM, p % 8)) = v;
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * T::kThreads, r = i / (D / 8), p = i % (D / 8);
+        const uint4 y = paired_order(v[x]);
+        if (i < NQ * kM * (D / 8))
+          *reinterpret_cast<uint4*>(smem + (r / kM) * T::kQBytes + (p / 8) * (kM * 128) + panel_piece(r % kM, p % 8)) =
+              make_uint4((y.x ^ flip) & keep, (y.y ^ flip) & keep, (y.z ^ flip) & keep, (y.w ^ flip) & keep);
+      }
     }
   }
-  for (int i = tid; i < 2 * kN; i += T::kThreads) *reinterpret_cast<uint32_t*>(s_bad[i / kN][i % kN]) = 0;
-  if (warp == kMmaWarp) {
+  for (int i = tid; i < 2 * kN; i += T::kThreads) *reinterpret_cast<uint2*>(s_bad[i / kN][i % kN]) = make_uint2(0, 0);
+  if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(bar(kKFull + i), T::kFill);
-        mbar_init(bar(kKEmpty + i), 1);
+        mbar_init(bar(kKEmpty + i), NQ);
         mbar_init(bar(kVFull + i), T::kFill);
-        mbar_init(bar(kVEmpty + i), 1);
+        mbar_init(bar(kVEmpty + i), NQ);
         mbar_init(bar(kSFull + i), 1);
         mbar_init(bar(kPFull + i), kM);
         mbar_init(bar(kOFull + i), 1);
@@ -234,30 +258,47 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     const int lim = s_limit[r];
     const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
     float m = -INFINITY, l = 0.0f;  // m: of the unscaled scores, as of the last rescale
-    uint32_t bad = 0;
+    uint32_t bad = 0;  // bit g: group g of v
     bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
+    // Products, by the tile's first thread.  They run in the order of their issue.
+    const bool issuer = (warp & 3) == 0 && lane == 0;
+    constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
+    auto scores = [&](int j) {  // S of tile j; false if its keys do not come
+      if (!mbar_wait_bounded(bar(kKFull + (j & 1)), (j >> 1) & 1)) return;
+      tcgen05_after_sync();
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        tcgen05_mma(tmem + qt * kN, panel_desc(base + T::kQ + qt * T::kQBytes + (k / 4) * (kM * 128) + 32 * (k % 4)),
+                    panel_desc(base + T::kK + (j & 1) * T::kKBytes + (k / 4) * (kN * 128) + 32 * (k % 4)), kShapeS,
+                    k > 0);
+      tcgen05_commit(bar(kSFull + qt));
+      tcgen05_commit(bar(kKEmpty + (j & 1)));
+    };
+    if (issuer && n > 0) scores(0);
+    __syncwarp();
+    for (int j = 0; j < n; ++j) {
       const int first = (j0 + j) * kN;
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kSFull + qt), j & 1));
       if (!ok) break;
       tcgen05_after_sync();
-      const bool whole = __all_sync(0xffffffffu, first + kN <= lim);  // no masked score in the warp's rows
-      float top = -INFINITY;
+      uint32_t s[kN];
 #pragma unroll
-      for (int c = 0; c < kN / 32; ++c) {
-        uint32_t s[32];
-        tmem_load32(s, s_at + 32 * c);
-        tmem_wait_load();
-        if (whole) {
-          float x[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+      for (int c = 0; c < kN / 32; ++c) tmem_load32(s + 32 * c, s_at + 32 * c);
+      tmem_wait_load<kN>(s);
+      if (!__all_sync(0xffffffffu, first + kN <= lim)) {  // some score of the warp's rows is masked
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i & 3] = max_nan(x[i & 3], __uint_as_float(s[i]));
-          top = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
-        } else {
+        for (int i = 0; i < kN; ++i)
+          if (first + i >= lim) s[i] = 0xff800000u;
+      }
+      float top;
+      {
+        float x[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (first + 32 * c + i < lim) top = max_nan(top, __uint_as_float(s[i]));
-        }
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(s[i]);
+#pragma unroll
+        for (int i = 4; i + 1 < kN; i += 2)
+          x[(i >> 1) & 3] = max3_nan(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        top = max3_nan(x[0], x[1], max_nan(x[2], x[3]));
       }
       // Grown by more than the slack (or from nothing, or NaN): rescale.  S of this
       // tile is complete, so every product issued before it is, O's among them.
@@ -272,52 +313,64 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         if (j > 0) {
           const float by = grown ? f : 1.0f;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_load32(o, o_at + 32 * c);
-            tmem_wait_load();
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_load16(o, o_at + 16 * c);
+            tmem_wait_load<16>(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-            tmem_store32(o_at + 32 * c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+            tmem_store16(o_at + 16 * c, o);
           }
         }
       }
       const float shift = m == -INFINITY ? 0.0f : m * scale;
-      float sum[2] = {0.0f, 0.0f};
+      const uint64_t scale2 = pack_f32x2(__float_as_uint(scale), __float_as_uint(scale));
+      const uint64_t shift2 = pack_f32x2(__float_as_uint(-shift), __float_as_uint(-shift));
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < kN / 32; ++c) {
-        uint32_t s[32], p[16];
-        tmem_load32(s, s_at + 32 * c);
-        tmem_wait_load();
+        uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float x = exp2_approx(fmaf(__uint_as_float(s[2 * i]), scale, -shift));
-          float y = exp2_approx(fmaf(__uint_as_float(s[2 * i + 1]), scale, -shift));
-          if (!whole) {
-            if (first + 32 * c + 2 * i >= lim) x = 0.0f;
-            if (first + 32 * c + 2 * i + 1 >= lim) y = 0.0f;
-          }
-          sum[i & 1] += x + y;
-          p[i] = pack_bf16x2(x, y);
+          const uint64_t y = fma_f32x2(pack_f32x2(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), scale2, shift2);
+          const float p0 = exp2_approx(lo_f32(y)), p1 = exp2_approx(hi_f32(y));
+          sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
+          p[i] = pack_bf16x2(p0, p1);
         }
-        tmem_store16(s_at + 16 * c, p);  // columns whose scores have been read
+        tmem_store16(s_at + 16 * c, p);  // over scores that this thread has in registers
       }
       tmem_wait_store();
       tcgen05_before_sync();
       mbar_arrive(bar(kPFull + qt));
-      l += sum[0] + sum[1];
+      const uint64_t both = add_f32x2(sum[0], sum[1]);
+      l += lo_f32(both) + hi_f32(both);
+      if (issuer && mbar_wait_bounded(bar(kPFull + qt), j & 1) &&
+          mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1)) {
+        tcgen05_after_sync();
+#pragma unroll
+        for (int k = 0; k < kN / 16; ++k)
+          tcgen05_mma_ta(tmem + NQ * kN + qt * D, tmem + qt * kN + 8 * k,
+                         panel_desc(base + T::kV + (j & 1) * T::kVBytes + (k / 4) * (D * 128) + 32 * (k % 4)), kShapeO,
+                         j > 0 || k > 0);
+        tcgen05_commit(bar(kVEmpty + (j & 1)));
+        if (j + 1 < n)
+          scores(j + 1);  // replaces P, which the products before it have read by then
+        else
+          tcgen05_commit(bar(kOFull + qt));
+      }
+      __syncwarp();
       if (first + kN > lowest && lowest < limit) {
         // rows that some query must not see: the groups of v that are not finite were read as zeros
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1));
         if (!ok) break;
-        const uint4* flags = reinterpret_cast<const uint4*>(s_bad[j & 1]);
-        for (int i = 0; i < kN / 4; ++i) {
-          const uint4 f = flags[i];
-          if ((f.x | f.y | f.z | f.w) == 0) continue;
+        const uint2* flags = reinterpret_cast<const uint2*>(s_bad[j & 1]);
+        for (int i = 0; i < kN && first + i < lim; ++i) {
+          const uint2 f = flags[i];
+          if ((f.x | f.y) == 0) continue;
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-            if (first + 4 * i + w < lim) bad |= vget(f, w);
+          for (int x = 0; x < 4; ++x) bad |= (f.x >> (8 * x) & 1u) << x | (f.y >> (8 * x) & 1u) << (4 + x);
         }
+        __syncwarp();
       }
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kOFull + qt), 0));
@@ -328,19 +381,19 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     if (split.count == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (row < rows && a.lse != nullptr)
-        a.lse[((int64_t)b * a.heads + head) * a.seq + sq] = m == -INFINITY ? -INFINITY : m * scale + log2f(l);
+        a.lse[q_row0() + row] = m == -INFINITY ? -INFINITY : m * scale + log2f(l);
       const int64_t at = (((int64_t)b * a.seq + sq) * a.heads + head) * D;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         if (n > 0) {
           tmem_load32(o, o_at + 32 * c);
-          tmem_wait_load();
+          tmem_wait_load<32>(o);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0;
         }
-        const bool nan = bad >> (8 * c) & 1u;
+        const bool nan = bad >> c & 1u;
 #pragma unroll
         for (int i = 0; i < 4 && row < rows && ok; ++i) {
           uint4 y, gate = make_uint4(0, 0, 0, 0);
@@ -365,18 +418,16 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       for (int c = 0; c < D / 32 && n > 0; ++c) {
         uint32_t o[32];
         tmem_load32(o, o_at + 32 * c);
-        tmem_wait_load();
+        tmem_wait_load<32>(o);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          reinterpret_cast<uint4*>(part + (int64_t)r * D + 32 * c)[i] =
-              make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        for (int i = 0; i < 32; ++i) part[(32 * c + i) * (NQ * kM) + r] = __uint_as_float(o[i]);
       }
       float* tail = part + NQ * kM * D + r;
       tail[0] = m == -INFINITY ? -INFINITY : m * scale;  // log2 units
       tail[NQ * kM] = l;
       tail[2 * NQ * kM] = __uint_as_float(bad);
     }
-  } else if (warp < kMmaWarp) {
+  } else {
     // --------------------------------------------------------------- filling
     const int t = tid - T::kSoftmax;
     const int64_t head_row = (int64_t)bh * a.c.cache_len;
@@ -384,7 +435,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     const uint8_t* vc = a.c.v_codes + head_row * (D / 2);
     const uint32_t* ks = a.c.k_scales + head_row * T::kGroups;
     const uint32_t* vs = a.c.v_scales + head_row * T::kGroups;
-    Codes<D> c;
+    Codes<D, kN> c;
     if (n > 0) {
       c.fetch_k(kc, ks, j0 * kN, limit, t);
       c.fetch_v(vc, vs, j0 * kN, limit, t);
@@ -403,116 +454,292 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       mbar_arrive(bar(kVFull + s));
       if (j + 1 < n) c.fetch_v(vc, vs, first + kN, limit, t);
     }
-  } else if (lane == 0) {
-    // -------------------------------------------------------------- products
-    constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
-    auto scores = [&](int q, int s) {
+  }
+  __syncwarp();
+  tcgen05_before_sync();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, T::kColumns);
+}
+
+// Joins the split items' partial results: a thread per query row and 16 elements.
+constexpr int kJoinElements = 16;
+template <int D, int NQ>
+__global__ void __launch_bounds__(kM) kv4_prefill_join_kernel(const AttnArgs a, const PrefillSplit split,
+                                                              const int blocks_q) {
+  grid_dependency_begin();
+  constexpr int kRows = NQ * kM, kCuts = D / kJoinElements;
+  const unsigned rows = a.group * a.seq;
+  const unsigned tile = blockIdx.x / kCuts, item = tile / NQ;  // query tile of 128 rows
+  const int d0 = (int)(blockIdx.x - tile * kCuts) * kJoinElements, r = (int)(tile - item * NQ) * kM + threadIdx.x;
+  const unsigned heads_all = (unsigned)(a.batch * a.kv_heads), back = item / heads_all;
+  const int bh = (int)(item - back * heads_all), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
+  const unsigned row = (blocks_q - 1 - back) * kRows + r;
+  if (row >= rows) return;
+  const float* parts = split.parts + (int64_t)item * split.count * prefill_part(NQ, D);
+  auto tail = [&](int i) -> const float* { return parts + i * prefill_part(NQ, D) + kRows * D + r; };
+  // online over the parts; the loads of 4 parts are in flight at once
+  constexpr int kAhead = 4;
+  float top = -INFINITY, norm = 0.0f, sum[kJoinElements];
+  uint32_t bad = 0;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = (k / 4) * (kM * 128) + 32 * (k % 4);
-        tcgen05_mma(tmem + q * kN, panel_desc(base + T::kQ + q * T::kQBytes + at),
-                    panel_desc(base + T::kK + s * T::kKBytes + at), kShapeS, k > 0);
-      }
-      tcgen05_commit(bar(kSFull + q));
-    };
-    bool ok = n > 0 && mbar_wait_bounded(bar(kKFull), 0);
-    if (ok) {
-      tcgen05_after_sync();
-      for (int q = 0; q < NQ; ++q) scores(q, 0);
-      tcgen05_commit(bar(kKEmpty));
+  for (int x = 0; x < kJoinElements; ++x) sum[x] = 0.0f;
+  for (int i0 = 0; i0 < split.count; i0 += kAhead) {
+    float m[kAhead], l[kAhead], v[kAhead][kJoinElements];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const bool in = i0 + i < split.count;
+      const float* t = tail(in ? i0 + i : 0);
+      const float* part = parts + (in ? i0 + i : 0) * prefill_part(NQ, D) + d0 * kRows + r;
+      m[i] = in ? t[0] : -INFINITY;
+      l[i] = t[kRows];
+      if (in) bad |= __float_as_uint(t[2 * kRows]);
+#pragma unroll
+      for (int x = 0; x < kJoinElements; ++x) v[i][x] = part[x * kRows];
     }
-    for (int j = 0; j < n && ok; ++j) {
-      const int s = j & 1, next = (j + 1) & 1;
-      ok = mbar_wait_bounded(bar(kVFull + s), (j >> 1) & 1);
-      for (int q = 0; q < NQ && ok; ++q) {
-        ok = mbar_wait_bounded(bar(kPFull + q), j & 1);
-        if (!ok) break;
-        tcgen05_after_sync();
+    float now = top;
 #pragma unroll
-        for (int k = 0; k < kN / 16; ++k)
-          tcgen05_mma_ta(tmem + NQ * kN + q * D, tmem + q * kN + 8 * k,
-                         panel_desc(base + T::kV + s * T::kVBytes + (k / 4) * (D * 128) + 32 * (k % 4)), kShapeO,
-                         j > 0 || k > 0);
-        // the next scores replace P once it has been read: products run in the order of their issue
-        if (j + 1 < n) {
-          if (q == 0) ok = mbar_wait_bounded(bar(kKFull + next), ((j + 1) >> 1) & 1);
-          if (!ok) break;
-          tcgen05_after_sync();
-          scores(q, next);
+    for (int i = 0; i < kAhead; ++i) now = max_nan(now, m[i]);
+    const float back_by = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+    norm *= back_by;
+#pragma unroll
+    for (int x = 0; x < kJoinElements; ++x) sum[x] *= back_by;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (m[i] == -INFINITY) continue;  // a part without rows left only this mark
+      const float f = exp2_approx(m[i] - now);
+      norm += f * l[i];
+#pragma unroll
+      for (int x = 0; x < kJoinElements; ++x) sum[x] += f * v[i][x];
+    }
+    top = now;
+  }
+  const unsigned g = row / a.seq, s = row - g * a.seq;
+  const int64_t head = hk * a.group + g;
+  if (a.lse != nullptr && d0 == 0)
+    a.lse[((int64_t)b * a.heads + hk * a.group) * a.seq + row] = top == -INFINITY ? -INFINITY : top + log2f(norm);
+  const float inv = norm == 0.0f ? 0.0f : 1.0f / norm;
+  const bool nan = bad >> (d0 / kKv4Group) & 1u;
+  const int64_t at = (((int64_t)b * a.seq + s) * a.heads + head) * D + d0;
+#pragma unroll
+  for (int i = 0; i < kJoinElements / 8; ++i) {
+    uint4 y, gate = make_uint4(0, 0, 0, 0);
+    if (a.gate != nullptr) gate = ld_l2(reinterpret_cast<const uint4*>(a.gate + at) + i);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float v0 = sum[8 * i + 2 * w] * inv, v1 = sum[8 * i + 2 * w + 1] * inv;
+      if (nan) v0 = v1 = __int_as_float(0x7fc00000);
+      if (a.gate != nullptr) {
+        v0 *= 1.0f / (1.0f + __expf(-bf16_lo(vget(gate, w))));
+        v1 *= 1.0f / (1.0f + __expf(-bf16_hi(vget(gate, w))));
+      }
+      vset(y, w, pack_bf16x2(v0, v1));
+    }
+    st_l2(reinterpret_cast<uint4*>(a.out + at) + i, y);
+  }
+}
+
+// weights[j] += the probabilities of cache row j, summed over the query rows in
+// their order: S^T = K Q^T, recomputed, so that a thread has a cache row and sums
+// over its columns by itself -- no atomics, no shuffles, the same sum from call to
+// call.  A CTA owns 128 cache rows, dequantised once; 4 warps copy the query tiles
+// to shared memory (cp.async, two stages), one thread issues the products into two
+// buffers of tensor memory, 4 warps take the exponentials, 128 per row and tile,
+// which bound it.  Up to head_dim 128 two CTAs share an SM.
+template <int D>
+struct Wgt {
+  static constexpr int kK = 0, kBytes = 128 * D * 2, kQ = kBytes;  // keys; two stages of queries
+  // (at least so much that no third CTA comes to an SM, whose tensor memory two fill)
+  static constexpr int kSmem = D == 64 ? 80 * 1024 : 3 * kBytes + 1024;
+  static constexpr int kThreads = 128 + 128 + 32;
+  static constexpr uint32_t kColumns = 256;
+};
+enum { kWFull = 0, kWEmpty = 2, kWSFull = 4, kWSEmpty = 6, kWBars = 8 };
+
+// Query rows [128 i, + 128) of a kv head: the highest and the lowest number of cache
+// rows that one of them sees (rows past the last: none).
+__device__ __forceinline__ int2 tile_limits(const AttnArgs& a, int b, unsigned rows, int i) {
+  const unsigned r0 = i * 128u, r1 = min(r0 + 127, rows - 1), seq = a.seq;
+  const unsigned g0 = r0 / seq, s0 = r0 - g0 * seq, g1 = r1 / seq, s1 = r1 - g1 * seq;
+  return make_int2(visible_rows(a, b, (int)(g0 == g1 ? s1 : seq - 1)),
+                   r0 + 127 >= rows ? 0 : visible_rows(a, b, (int)(g0 == g1 ? s0 : 0)));
+}
+
+template <int D>
+__global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const AttnArgs a, const int tiles_k) {
+  using T = Wgt<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[kWBars];
+  __shared__ uint32_t s_tmem;
+  __shared__ __align__(16) float s_lse[4][128];  // negated
+  __shared__ int s_lim[4][128];
+  uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8 * i; };
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_begin();
+  const unsigned rows = a.group * a.seq;
+  const int bh = (int)(blockIdx.x / (unsigned)tiles_k), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
+  const int first = (int)(blockIdx.x - bh * tiles_k) * 128;
+  const int limit = visible_rows(a, b, a.seq - 1);  // of the last query: the highest
+  if (first >= limit) return;
+  const int tiles_q = (int)((rows + 127) / 128);
+
+  const int64_t head_row = (int64_t)bh * a.c.cache_len;
+  {  // the keys, elements in kv4_pair's order put back: the queries are copied as they are
+    const uint8_t* kc = a.c.k_codes + head_row * (D / 2);
+    const uint32_t* ks = a.c.k_scales + head_row * (D / 32);
+    for (int i = tid; i < 128 * (D / 32); i += T::kThreads) {
+      const int row = i / (D / 32), p = i % (D / 32);
+      uint4 c = make_uint4(0, 0, 0, 0);
+      uint32_t sz = 0;
+      if (first + row < limit) {
+        c = ld_l2(reinterpret_cast<const uint4*>(kc + (int64_t)(first + row) * (D / 2)) + p);
+        sz = __ldcg(ks + (int64_t)(first + row) * (D / 32) + p);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int at = 4 * p + w;
+        *reinterpret_cast<uint4*>(smem + T::kK + (at / 8) * (128 * 128) + panel_piece(row, at % 8)) =
+            kv4_values(vget(c, w), sz);
+      }
+    }
+  }
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(bar(kWFull + i), 128);
+        mbar_init(bar(kWEmpty + i), 1);
+        mbar_init(bar(kWSFull + i), 1);
+        mbar_init(bar(kWSEmpty + i), 128);
+      }
+      mbar_init_fence();
+    }
+    __syncwarp();
+    tmem_alloc(smem_addr(&s_tmem), T::kColumns);
+  }
+  fence_proxy_async_smem();
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  const uint32_t tmem = s_tmem;
+
+  if (warp < 4) {
+    // ----------------------------------------------------------- probabilities
+    const int at = first + tid;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    uint64_t sum[2] = {0, 0};
+    float extra = 0.0f;  // of tiles with masked probabilities
+    const uint64_t scale2 = pack_f32x2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
+    int n = 0;
+    for (int i = 0; i < tiles_q; ++i) {
+      const int2 see = tile_limits(a, b, rows, i);
+      if (see.x <= first) continue;
+      const int s = n & 1, phase = (n >> 1) & 1, entry = n & 3;
+      ++n;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(kWSFull + s), phase))) break;
+      tcgen05_after_sync();
+      const bool whole = first + 128 <= see.y;
+      uint32_t x[2][32];  // 32 columns are loaded while the 32 before them are worked on
+      tmem_load32(x[0], tmem + lanes + 128 * s);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_wait_load<32>(x[c & 1]);
+        if (c < 3) tmem_load32(x[(c + 1) & 1], tmem + lanes + 128 * s + 32 * (c + 1));
+        if (whole) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint4 lse = *reinterpret_cast<const uint4*>(&s_lse[entry][32 * c + 4 * q]);
+            const uint64_t y0 = fma_f32x2(pack_f32x2(x[c & 1][4 * q], x[c & 1][4 * q + 1]), scale2, pack_f32x2(lse.x, lse.y));
+            const uint64_t y1 = fma_f32x2(pack_f32x2(x[c & 1][4 * q + 2], x[c & 1][4 * q + 3]), scale2, pack_f32x2(lse.z, lse.w));
+            sum[0] = add_f32x2(sum[0], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y0))), __float_as_uint(exp2_approx(hi_f32(y0)))));
+            sum[1] = add_f32x2(sum[1], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y1))), __float_as_uint(exp2_approx(hi_f32(y1)))));
+          }
         } else {
-          tcgen05_commit(bar(kOFull + q));
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (at < s_lim[entry][32 * c + q])
+              extra += exp2_approx(fmaf(__uint_as_float(x[c & 1][q]), a.scale_log2, s_lse[entry][32 * c + q]));
         }
       }
-      if (!ok) break;
-      tcgen05_commit(bar(kVEmpty + s));
-      if (j + 1 < n) tcgen05_commit(bar(kKEmpty + next));
+      tcgen05_before_sync();
+      mbar_arrive(bar(kWSEmpty + s));
+    }
+    const uint64_t both = add_f32x2(sum[0], sum[1]);
+    if (at < limit) a.c.weights[head_row + at] += lo_f32(both) + hi_f32(both) + extra;
+  } else if (warp < 8) {
+    // ----------------------------------------------------------------- queries
+    const int t = tid - 128;
+    const int64_t q_row0 = ((int64_t)b * a.heads + hk * a.group) * a.seq;  // the head's query rows lie one after another
+    const uint4* src = a.q + q_row0 * (D / 8);
+    auto fetch = [&](int i, int s) {
+      const int64_t at = (int64_t)i * (128 * (D / 8));
+#pragma unroll
+      for (int x = t; x < 128 * (D / 8); x += 128) {
+        const int r = x / (D / 8), p = x % (D / 8);
+        const bool in = i * 128u + r < rows;
+        cp_async_zfill<16>(base + T::kQ + s * T::kBytes + (p / 8) * (128 * 128) + panel_piece(r, p % 8),
+                           in ? src + at + x : src, in);
+      }
+    };
+    int n = 0;
+    for (int i = 0; i < tiles_q; ++i) {
+      if (tile_limits(a, b, rows, i).x <= first) continue;
+      const int s = n & 1, phase = (n >> 1) & 1;
+      if (!mbar_wait_bounded(bar(kWEmpty + s), phase ^ 1)) break;
+      fetch(i, s);
+      cp_async_commit();
+      // (entry n & 3 of lse and limits: its last reader freed the scores' buffer that the
+      // products of tile n - 2, now done, went to)
+      const unsigned row = i * 128u + t;
+      s_lse[n & 3][t] = row < rows ? -a.lse[q_row0 + row] : 0.0f;
+      s_lim[n & 3][t] = row < rows ? visible_rows(a, b, (int)(row % (unsigned)a.seq)) : -1;
+      ++n;
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      mbar_arrive(bar(kWFull + s));
+    }
+  } else if (lane == 0) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t kShape = mma_shape(128, 128);
+    int n = 0;
+    for (int i = 0; i < tiles_q; ++i) {
+      if (tile_limits(a, b, rows, i).x <= first) continue;
+      const int s = n & 1, phase = (n >> 1) & 1;
+      ++n;
+      if (!mbar_wait_bounded(bar(kWFull + s), phase) || !mbar_wait_bounded(bar(kWSEmpty + s), phase ^ 1)) break;
+      tcgen05_after_sync();
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t from = (k / 4) * (128 * 128) + 32 * (k % 4);
+        tcgen05_mma(tmem + 128 * s, panel_desc(base + T::kK + from), panel_desc(base + T::kQ + s * T::kBytes + from),
+                    kShape, k > 0);
+      }
+      tcgen05_commit(bar(kWSFull + s));
+      tcgen05_commit(bar(kWEmpty + s));
     }
   }
   __syncwarp();
   tcgen05_before_sync();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_free(tmem, T::kColumns);
+  if (warp == 8) tmem_free(tmem, T::kColumns);
 }
 
-// Joins the split items' partial results: a warp per query row.
-template <int D, int NQ>
-__global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const AttnArgs a, const PrefillSplit split,
-                                                               const int blocks_q) {
-  grid_dependency_begin();
-  const unsigned rows = a.group * a.seq;
-  const unsigned line = blockIdx.x * 8 + threadIdx.x / 32;  // item * 128 NQ + r
-  const unsigned item = line / (NQ * kM), r = line % (NQ * kM);
-  const int bh = (int)(item / blocks_q), b = bh / a.kv_heads, hk = bh - b * a.kv_heads, lane = threadIdx.x & 31;
-  const unsigned row = (blocks_q - 1 - (item - bh * blocks_q)) * (NQ * kM) + r;
-  if (row >= rows) return;
-  const float* parts = split.parts + (int64_t)item * split.count * prefill_part(NQ, D);
-  float top = -INFINITY, norm = 0.0f;
-  uint32_t bad = 0;
-  for (int i = 0; i < split.count; ++i) top = max_nan(top, parts[i * prefill_part(NQ, D) + NQ * kM * D + r]);
-  float sum[D / 32];
-#pragma unroll
-  for (int x = 0; x < D / 32; ++x) sum[x] = 0.0f;
-  for (int i = 0; i < split.count; ++i) {
-    const float* part = parts + i * prefill_part(NQ, D);
-    const float m = part[NQ * kM * D + r];
-    if (m == -INFINITY) continue;
-    const float f = exp2_approx(m - top);
-    norm += f * part[NQ * kM * D + NQ * kM + r];
-    bad |= __float_as_uint(part[NQ * kM * D + 2 * NQ * kM + r]);
-#pragma unroll
-    for (int x = 0; x < D / 64; ++x) {
-      const float2 v = *reinterpret_cast<const float2*>(part + (int64_t)r * D + 64 * x + 2 * lane);
-      sum[2 * x] += f * v.x;
-      sum[2 * x + 1] += f * v.y;
-    }
-  }
-  const unsigned g = row / a.seq, s = row - g * a.seq;
-  const int64_t head = hk * a.group + g;
-  if (a.lse != nullptr && lane == 0)
-    a.lse[((int64_t)b * a.heads + head) * a.seq + s] = top == -INFINITY ? -INFINITY : top + log2f(norm);
-  const float inv = norm == 0.0f ? 0.0f : 1.0f / norm;
-  const int64_t at = (((int64_t)b * a.seq + s) * a.heads + head) * D;
-#pragma unroll
-  for (int x = 0; x < D / 64; ++x) {
-    const int d = 64 * x + 2 * lane;
-    float v0 = sum[2 * x] * inv, v1 = sum[2 * x + 1] * inv;
-    if (bad >> (8 * (d / kKv4Group)) & 1u) v0 = v1 = __int_as_float(0x7fc00000);
-    if (a.gate != nullptr) {
-      const uint32_t y = *reinterpret_cast<const uint32_t*>(a.gate + at + d);
-      v0 *= 1.0f / (1.0f + __expf(-bf16_lo(y)));
-      v1 *= 1.0f / (1.0f + __expf(-bf16_hi(y)));
-    }
-    *reinterpret_cast<uint32_t*>(a.out + at + d) = pack_bf16x2(v0, v1);
-  }
+template <int D>
+cudaError_t launch_weights(const AttnArgs& a, int64_t longest, cudaStream_t s) {
+  const int64_t tiles = (longest + 127) / 128, grid = a.batch * a.kv_heads * tiles;
+  if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const cudaError_t e = allow_shared<kv4_weights_kernel<D>>(Wgt<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kv4_weights_kernel<D>, grid, Wgt<D>::kThreads, Wgt<D>::kSmem, s, a, (int)tiles);
 }
 
 struct PrefillShape {
   int nq, blocks_q;
   int64_t items;
 };
-PrefillShape prefill_shape(int64_t batch_kv_heads, int64_t rows) {
+PrefillShape prefill_shape(int64_t batch_kv_heads, int64_t rows, int64_t head_dim) {
   PrefillShape s;
-  s.nq = rows > kM ? 2 : 1;
+  s.nq = rows > kM && head_dim <= 128 ? 2 : 1;
   s.blocks_q = (int)((rows + s.nq * kM - 1) / (s.nq * kM));
   s.items = batch_kv_heads * s.blocks_q;
   return s;
@@ -523,28 +750,44 @@ cudaError_t launch_prefill(const AttnArgs& a, const PrefillShape& p, int64_t lon
   using T = Pre<D, NQ>;
   // One CTA per SM: items that leave SMs idle are split, to 4 tiles at least.
   PrefillSplit split{1, parts};
-  while (p.items * (split.count + 1) <= device_sm_count() && (split.count + 1) * 4 * kN <= longest) ++split.count;
+  while (p.items * (split.count + 1) <= device_sm_count() && (split.count + 1) * 4 * T::kN <= longest) ++split.count;
   if (p.items * split.count > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaError_t e = allow_shared<kv4_prefill_kernel<D, NQ>>(T::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_kernel(kv4_prefill_kernel<D, NQ>, p.items * split.count, T::kThreads, T::kSmem, s, a, split, p.blocks_q);
   if (e != cudaSuccess || split.count == 1) return e;
-  return launch_kernel(kv4_prefill_join_kernel<D, NQ>, p.items * NQ * kM / 8, 256, 0, s, a, split, p.blocks_q);
+  return launch_kernel(kv4_prefill_join_kernel<D, NQ>, p.items * NQ * (D / kJoinElements), kM, 0, s, a, split,
+                       p.blocks_q);
 }
 
 }  // namespace
 
 int64_t kv4_prefill_workspace(int64_t batch_kv_heads, int64_t rows, int64_t head_dim) {
-  const PrefillShape p = prefill_shape(batch_kv_heads, rows);
+  const PrefillShape p = prefill_shape(batch_kv_heads, rows, head_dim);
   const int64_t most = device_sm_count() / (p.items > 0 ? p.items : 1);  // CTAs per item, for any cache length
   return most < 2 ? 0 : p.items * most * prefill_part(p.nq, head_dim) * (int64_t)sizeof(float);
 }
 
 cudaError_t launch_kv4_prefill(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s) {
-  const PrefillShape p = prefill_shape(a.batch * a.kv_heads, (int64_t)a.group * a.seq);
-  if (head_dim == 64)
-    return p.nq == 1 ? launch_prefill<64, 1>(a, p, longest, parts, s) : launch_prefill<64, 2>(a, p, longest, parts, s);
-  return p.nq == 1 ? launch_prefill<128, 1>(a, p, longest, parts, s) : launch_prefill<128, 2>(a, p, longest, parts, s);
+  const PrefillShape p = prefill_shape(a.batch * a.kv_heads, (int64_t)a.group * a.seq, head_dim);
+  switch (head_dim) {
+    case 64:
+      return p.nq == 1 ? launch_prefill<64, 1>(a, p, longest, parts, s) : launch_prefill<64, 2>(a, p, longest, parts, s);
+    case 128:
+      return p.nq == 1 ? launch_prefill<128, 1>(a, p, longest, parts, s)
+                       : launch_prefill<128, 2>(a, p, longest, parts, s);
+    case 192: return launch_prefill<192, 1>(a, p, longest, parts, s);
+    default: return launch_prefill<256, 1>(a, p, longest, parts, s);
+  }
+}
+
+cudaError_t launch_kv4_weights(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s) {
+  switch (head_dim) {
+    case 64: return launch_weights<64>(a, longest, s);
+    case 128: return launch_weights<128>(a, longest, s);
+    case 192: return launch_weights<192>(a, longest, s);
+    default: return launch_weights<256>(a, longest, s);
+  }
 }
 
 cudaError_t kv4_prefill_wait_timeouts(unsigned int* count, bool reset) {

@@ -130,7 +130,6 @@ cudaError_t launch_kv4_update(const void* k, const void* v, const Kv4View& c, in
 // bytes for the same sizes.
 int64_t kv4_decode_workspace(int64_t rows, int64_t head_dim, int64_t longest);
 cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s);
-cudaError_t launch_kv4_chunk(const AttnArgs& a, int64_t head_dim, cudaStream_t s);
 int64_t kv4_prefill_workspace(int64_t batch_kv_heads, int64_t rows, int64_t head_dim);
 cudaError_t launch_kv4_prefill(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s);
 cudaError_t kv4_prefill_wait_timeouts(unsigned int* count, bool reset);

@@ -127,7 +127,6 @@ def test_attention_workspace_sizes(lib):
     assert size(3, 1, 0, rows=4096) == 0
     assert size(3, 1, 0, rows=65536) > 0            # partial results of a split decode
     assert size(3, 33, 0, rows=65536, batch=200) == 0
-    assert size(3, 33, 0, rows=65536, dim=256) == 0
     assert lib.hrm_kv4_attention_workspace(cache(), 3, 2, 1, None) == code("NULL_POINTER")
 
 
