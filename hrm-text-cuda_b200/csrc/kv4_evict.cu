@@ -7,14 +7,15 @@
 // in-place eviction moves the fewest rows -- one per decode step -- and attention
 // over the cache, which is indifferent to the order of its rows, reads it as is.
 //
-// What bounds it: 8 bytes per row read (weight, position) and the rows moved;
-// small cases are bound by the latency of the selection.  The selection keeps
-// the keys in registers, as integers that order like them, and bisects on the
-// key's value with one CTA-wide count per step -- no sort, no atomics, and it
-// ends as soon as a threshold leaves exactly `budget` keys.  When a single row
-// must go (a decode step) it is a CTA-wide minimum instead.
-// The CTAs of a cluster select redundantly (the keys come from L2) and share the
-// rows to move; a cluster barrier separates reading the keys from moving rows.
+// What bounds it: 8 bytes per row read (weight, position) and the rows moved, by
+// bandwidth only in large batches; else by the latency of the selection's steps.
+// The CTAs of a cluster share a head's rows.  Keys stay in registers, as integers
+// that order like the weights; the budget-th largest is found digit by digit (11, 11
+// and 10 bits), each by counting in shared memory and adding up the cluster's counts
+// over distributed shared memory -- counts only, so their order changes nothing --
+// and ends early when a digit's border leaves exactly `budget` rows.  Rows whose key
+// is the threshold are then taken in row order.  When a single row must go (a
+// decode step) it is one CTA-wide minimum instead.
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -39,6 +40,9 @@ struct EvictArgs {
 };
 
 constexpr uint32_t kInfKey = 0xff800000u;
+constexpr uint32_t kAll = 0xffffffffu;
+constexpr int kBins = 2048;
+constexpr int kListed = 128;  // rows that a warp lists before it copies them
 
 // An integer that orders like the weight; 0 for NaN, kInfKey for +inf.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -47,238 +51,347 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the CTA, given to every thread; `buf` holds one word per warp.  Two
-// alternating buffers make one barrier per call enough.
+// Exclusive sum of x over the CTA's threads in order, and the total.  Two alternating
+// buffers of a word per warp make one barrier per call enough.
 template <int W>
-__device__ __forceinline__ int cta_sum(int x, int* buf) {
-  x = __reduce_add_sync(0xffffffffu, x);
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
-  __syncthreads();
-  int s = 0;
+__device__ __forceinline__ int cta_scan(int x, int* buf, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = x;
 #pragma unroll
-  for (int w = 0; w < W; ++w) s += buf[w];
-  return s;
+  for (int o = 1; o < 32; o *= 2) {
+    const int y = __shfl_up_sync(kAll, sum, o);
+    if (lane >= o) sum += y;
+  }
+  if (lane == 31) buf[warp] = sum;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const int y = buf[w];
+    all += y;
+    if (w < warp) before += y;
+  }
+  *total = all;
+  return before + sum - x;
 }
 
-// Words of shared memory: the moving rows in order, then a bit per place that
-// keeps its row and, per 32 places, how many are freed before them.
+// Rows that can move at most, and the dynamic shared memory: counts of the three
+// digits, the cluster's sums of one, per 32 rows of the CTA a mask and two ranks,
+// and the freed places in order (in the cluster's first CTA).
 inline int64_t evict_moves(int64_t n, int64_t budget) { return n <= budget ? 0 : (n - budget < budget ? n - budget : budget); }
 constexpr size_t kSharedMost = 200 * 1024;
-inline size_t evict_shared(int64_t n, int64_t budget) {
-  return 4 * (size_t)(evict_moves(n, budget) + 2 * ((budget + 31) / 32));
-}
+inline size_t evict_shared(int64_t groups, int64_t moves) { return 4 * (size_t)(4 * kBins + 3 * groups + moves); }
 
-// W warps; K keys per lane held in registers, or K = 0: read again at each use.
-// Warp w owns the rows [w * steps * 32, (w + 1) * steps * 32), 32 at a time, so
-// that ranks in row order need one CTA-wide step.
+// W warps per CTA; K steps of 32 rows per warp, their keys in registers (K = 0: any
+// number, the keys read again at each use).  CTA c of the cluster's `count` has the
+// rows [c, c + 1) * W * steps * 32; groups of 32 rows go to the warps in turn, so that the
+// copies are even over the warps wherever the rows that stay lie.
 template <int W, int K>
-__global__ void __launch_bounds__(W * 32) kv4_evict_kernel(const EvictArgs a, const int shares, const int moves_at_most) {
-  extern __shared__ int movers[];
-  uint32_t* keeps = reinterpret_cast<uint32_t*>(movers + moves_at_most);
-  int* freed = reinterpret_cast<int*>(keeps + (a.budget + 31) / 32);
+__global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2) kv4_evict_kernel(const EvictArgs a, const int count, const int steps_at_most) {
+  extern __shared__ __align__(16) int shared[];
+  int* hist = shared;                                                 // [3][kBins]
+  int* sums = shared + 3 * kBins;                                     // [kBins]: the cluster's
+  uint32_t* masks = reinterpret_cast<uint32_t*>(shared + 4 * kBins);  // per group: rows that stay
+  int* hole_at = shared + 4 * kBins + W * steps_at_most;              // freed places in the groups before
+  int* move_at = hole_at + W * steps_at_most;                         // moving rows in the groups before
+  int* freed = move_at + W * steps_at_most;                           // in the cluster's first CTA
   __shared__ int buf[2][32];
-  __shared__ int s_total[3][32];
+  __shared__ int s_totals[3];  // this CTA's rows equal to the threshold, freed places, moving rows
+  __shared__ int s_bin, s_above, s_in;
   __shared__ unsigned long long s_low[32];
+  __shared__ int2 s_copy[W][kListed];  // (source row, place)
   grid_dependency_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int share = blockIdx.x % shares;
-  const int64_t bh = blockIdx.x / shares, b = bh / a.kv_heads;
+  const unsigned head = count == 1 ? blockIdx.x : blockIdx.x / (unsigned)count;
+  const int rank = (int)(blockIdx.x - head * count);
+  const int64_t bh = head, b = bh / a.kv_heads;
   int64_t len = a.lengths ? a.lengths[b] : a.length;
   len = len < 0 ? 0 : (len > a.from.cache_len ? a.from.cache_len : len);
   const int n = (int)len, budget = a.budget, kept = n < budget ? n : budget;
   const int64_t protect = a.protect_froms ? a.protect_froms[b] : a.protect_from;
-  if (share == 0 && bh == b * a.kv_heads && threadIdx.x == 0) a.new_lengths[b] = kept;
+  if (rank == 0 && bh == b * a.kv_heads && threadIdx.x == 0) a.new_lengths[b] = kept;
   const float* weights = a.from.weights + bh * a.from.cache_len;
   const int* positions = a.from.positions + bh * a.from.cache_len;
+  cg::cluster_group cluster = cg::this_cluster();
+  auto join = [&]() {  // a barrier over the CTAs that share the head
+    if (count > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
 
-  const int steps = K > 0 ? K : (n + W * 32 - 1) / (W * 32);
-  const int base = warp * steps * 32 + lane;
+  const int steps = K > 0 ? K : (n + count * W * 32 - 1) / (count * W * 32);
+  const int cta_row = rank * W * steps * 32;           // the CTA's first row
+  auto row_of = [&](int i) -> int { return cta_row + (i * W + warp) * 32 + lane; };
+  auto make_key = [&](int row, int position, float weight) -> uint32_t {
+    return row >= n ? 0 : (position >= protect ? kInfKey : weight_key(weight));
+  };
   auto read_key = [&](int row) -> uint32_t {
-    return row >= n ? 0 : (positions[row] >= protect ? kInfKey : weight_key(weights[row]));
+    const int at = row < n ? row : 0;
+    return make_key(row, positions[at], weights[at]);
   };
   uint32_t reg[K > 0 ? K : 1];
   if (n > budget) {
+    int position[K > 0 ? K : 1];
+    float weight[K > 0 ? K : 1];
 #pragma unroll
-    for (int i = 0; i < K; ++i) reg[i] = read_key(base + 32 * i);
+    for (int i = 0; i < K; ++i) {  // all reads in flight at once
+      const int at = row_of(i) < n ? row_of(i) : 0;
+      position[i] = positions[at];
+      weight[i] = weights[at];
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i) reg[i] = make_key(row_of(i), position[i], weight[i]);
   }
-  auto key = [&](int i) -> uint32_t { return K > 0 ? reg[K > 0 ? i : 0] : read_key(base + 32 * i); };
+  auto key = [&](int i) -> uint32_t { return K > 0 ? reg[K > 0 ? i : 0] : read_key(row_of(i)); };
 
-  const bool single = n - budget == 1;
-  int out = -1;  // single: the row that goes
-  if (single) {
-    // the smallest key, of equal ones the last row
+  // A lane copies one 16-byte piece of codes (k, then v) and one word of scales of a
+  // row; `lanes` lanes (2 * code_pieces of them at work) make a row.
+  const int p = a.code_pieces, lanes = 2 * p <= 4 ? 4 : (2 * p <= 8 ? 8 : 16), sub = lane % lanes;
+  const bool works = sub < 2 * p, is_v = sub >= p;
+  const int64_t from0 = bh * a.from.cache_len, to0 = bh * a.to.cache_len;
+  const int piece = is_v ? sub - p : sub;
+  const uint4* code_from = reinterpret_cast<const uint4*>(is_v ? a.from.v_codes : a.from.k_codes) + from0 * p + piece;
+  const uint32_t* scale_from = (is_v ? a.from.v_scales : a.from.k_scales) + from0 * p + piece;
+  uint4* code_to = reinterpret_cast<uint4*>(is_v ? a.to.v_codes : a.to.k_codes) + to0 * p + piece;
+  uint32_t* scale_to = (is_v ? a.to.v_scales : a.to.k_scales) + to0 * p + piece;
+
+  if (n <= budget && a.in_place) return;  // the whole cluster
+  if (count == 1 && a.in_place && n - budget == 1) {
+    // One row goes: the smallest key, of equal ones the last row; the last row takes its place.
     unsigned long long low = ~0ull;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
-      const int row = base + 32 * i;
+      const int row = row_of(i);
       const unsigned long long x = (unsigned long long)key(i) << 32 | (uint32_t)(n - 1 - row);
       if (row < n && x < low) low = x;
     }
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) {
-      const unsigned long long x = __shfl_xor_sync(0xffffffffu, low, o);
+      const unsigned long long x = __shfl_xor_sync(kAll, low, o);
       low = x < low ? x : low;
     }
     if (lane == 0) s_low[warp] = low;
     __syncthreads();
+    if (warp > 0) return;
 #pragma unroll
     for (int w = 0; w < W; ++w) low = s_low[w] < low ? s_low[w] : low;
-    out = n - 1 - (int)(uint32_t)low;
-  } else if (n > budget) {
-    // bisect: count(key >= lo) >= budget > count(key >= hi); mid >= 1, so the keys
-    // 0 past the last row never count
-    uint64_t lo = 0, hi = 1ull << 32;
-    int above = 0, at_lo = n, turn = 0;
-    while (hi - lo > 1 && at_lo != budget) {
-      const uint32_t mid = (uint32_t)((lo + hi) / 2);
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < steps; ++i) c += key(i) >= mid;
-      c = cta_sum<W>(c, buf[turn]);
-      turn ^= 1;
-      if (c >= budget) {
-        lo = mid;
-        at_lo = c;
-      } else {
-        hi = mid;
-        above = c;
+    const int out = n - 1 - (int)(uint32_t)low;
+    if (out < budget) {
+      if (lane < lanes && works) {
+        code_to[(int64_t)out * p] = code_from[(int64_t)(n - 1) * p];
+        scale_to[(int64_t)out * p] = scale_from[(int64_t)(n - 1) * p];
+      }
+      if (lane == 0) {
+        a.to.weights[to0 + out] = weights[n - 1];
+        a.to.positions[to0 + out] = positions[n - 1];
       }
     }
-    // all keys >= lo stay; or those above it and, in row order, as many equal to it as there is room for
-    const bool exact = at_lo == budget;
-    const uint32_t threshold = (uint32_t)lo;
-    const int room = budget - above;
-    int eq = 0;  // keys equal to the threshold in earlier rows
-    if (!exact) {
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < steps; ++i)
-        c += __popc(__ballot_sync(0xffffffffu, base + 32 * i < n && key(i) == threshold));
-      if (lane == 0) s_total[0][warp] = c;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) eq += s_total[0][w];
-    }
-    // Per 32 rows the mask of those that stay.  It goes to shared memory for places;
-    // for rows past them the counts give the moving rows' ranks.
-    int holes = 0, moves = 0;
-    uint32_t mine = 0;  // lane i keeps the mask of step i (K > 0 has at most 32 steps)
-#pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int row = base + 32 * i, first = row - lane;
-      const uint32_t k = key(i);
-      uint32_t mask;
-      if (exact) {
-        mask = __ballot_sync(0xffffffffu, row < n && k >= threshold);
-      } else {
-        const uint32_t same = __ballot_sync(0xffffffffu, row < n && k == threshold);
-        const bool stays = row < n && (k > threshold || (k == threshold && eq + __popc(same & ((1u << lane) - 1)) < room));
-        eq += __popc(same);
-        mask = __ballot_sync(0xffffffffu, stays);
-      }
-      const int places = budget - first;  // of these 32 rows, the first ones that are places
-      const uint32_t low = places >= 32 ? 0xffffffffu : (places <= 0 ? 0u : (1u << places) - 1);
-      if (K > 0) mine = lane == i ? mask : mine;
-      if (lane == 0 && low != 0) {
-        keeps[first / 32] = mask;
-        freed[first / 32] = holes;  // within this warp's rows: completed below
-      }
-      holes += __popc(~mask & low);
-      moves += __popc(mask & ~low);
-    }
-    if (lane == 0) {
-      s_total[1][warp] = holes;
-      s_total[2][warp] = moves;
-    }
-    __syncthreads();
-    int hole = 0, move = 0;
-    for (int w = 0; w < warp; ++w) {
-      hole += s_total[1][w];
-      move += s_total[2][w];
-    }
-    if (!exact) {  // the equal keys' ranks again
-      eq = 0;
-      for (int w = 0; w < warp; ++w) eq += s_total[0][w];
-    }
-#pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int row = base + 32 * i, first = row - lane;
-      uint32_t mask;
-      if (K > 0) {
-        mask = __shfl_sync(0xffffffffu, mine, i);
-      } else {
-        const uint32_t k = key(i);
-        const uint32_t same = __ballot_sync(0xffffffffu, row < n && k == threshold);
-        mask = __ballot_sync(0xffffffffu, row < n && (k > threshold || (k == threshold &&
-                                              (exact || eq + __popc(same & ((1u << lane) - 1)) < room))));
-        eq += __popc(same);
-      }
-      const int places = budget - first;
-      const uint32_t low = places >= 32 ? 0xffffffffu : (places <= 0 ? 0u : (1u << places) - 1);
-      const uint32_t moving = mask & ~low;
-      if (moving >> lane & 1u) movers[move + __popc(moving & ((1u << lane) - 1))] = row;
-      move += __popc(moving);
-      if (lane == 0 && low != 0) freed[first / 32] += hole;
-    }
-  }
-  __syncthreads();
-  // In place, no CTA of this head may move a row while another still reads keys.
-  if (shares > 1 && a.in_place) cg::this_cluster().sync();
-  if (a.in_place && n <= budget) return;
-
-  // Copies: a lane moves one 16-byte piece of codes (k, then v) and one word of
-  // scales of a row; 2 * code_pieces lanes (rounded up to `lanes`) make a row.
-  const int p = a.code_pieces, lanes = 2 * p <= 4 ? 4 : (2 * p <= 8 ? 8 : 16);
-  const int per_warp = 32 / lanes, sub = lane % lanes;
-  const int first = (share * W + warp) * per_warp + lane / lanes;
-  auto source = [&](int d) -> int {
-    if (n <= budget) return d;
-    if (single) return d == out ? n - 1 : d;
-    const uint32_t m = keeps[d / 32];
-    if (m >> (d & 31) & 1u) return d;
-    return movers[freed[d / 32] + __popc(~m & ((1u << (d & 31)) - 1))];
-  };
-  auto copy = [&](int d, int src) {
-    const int64_t x = bh * a.from.cache_len + src, y = bh * a.to.cache_len + d;
-    if (sub < 2 * p) {
-      const bool v = sub >= p;
-      const int c = v ? sub - p : sub;
-      const uint4* from = reinterpret_cast<const uint4*>(v ? a.from.v_codes : a.from.k_codes) + x * p + c;
-      uint4* to = reinterpret_cast<uint4*>(v ? a.to.v_codes : a.to.k_codes) + y * p + c;
-      const uint32_t* sf = (v ? a.from.v_scales : a.from.k_scales) + x * p + c;
-      uint32_t* st = (v ? a.to.v_scales : a.to.k_scales) + y * p + c;
-      const uint4 code = *from;
-      const uint32_t scale = *sf;
-      *to = code;
-      *st = scale;
-    }
-    if (sub == 0) a.to.weights[y] = a.from.weights[x];
-    if (sub == 1) a.to.positions[y] = a.from.positions[x];
-  };
-  if (single && a.in_place) {
-    if (out < budget && share == 0 && warp == 0 && lane < lanes) copy(out, n - 1);
     return;
   }
-#pragma unroll 4
-  for (int d = first; d < kept; d += shares * W * per_warp) {
-    const int src = source(d);
-    if (!a.in_place || src != d) copy(d, src);
+
+  uint32_t threshold = 0;
+  bool exact = true;  // all keys >= threshold stay (n <= budget: all rows)
+  int room = 0;       // else: keys above it, and as many equal ones, in row order
+  if (n > budget) {
+    for (int i = threadIdx.x; i < 3 * kBins; i += W * 32) hist[i] = 0;
+    __syncthreads();
+    room = budget;
+    uint32_t prefix = 0, known = 0;  // the threshold's digits so far
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0), bins = d == 2 ? 1024 : kBins;
+      int* h = hist + d * kBins;
+#pragma unroll
+      for (int i = 0; i < steps; ++i) {
+        const uint32_t k = key(i);
+        if (row_of(i) < n && (k & known) == prefix) atomicAdd(&h[k >> shift & (bins - 1)], 1);
+      }
+      join();
+      // The cluster's sums: each CTA adds up its slice of the bins and gives it to the
+      // others (all CTAs adding up all bins moved four times as much).
+      const int* total = h;
+      if (count > 1) {
+        const int slice = bins / count;
+        for (int x = threadIdx.x; x < slice; x += W * 32) {
+          const int bin = rank * slice + x;
+          int y = 0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c < count) y += *cluster.map_shared_rank(&h[bin], c);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c < count) *cluster.map_shared_rank(&sums[bin], c) = y;
+        }
+        join();
+        total = sums;
+      }
+      // each thread: its consecutive bins, highest first
+      constexpr int kMost = kBins / (W * 32);
+      const int each = d == 2 ? kMost / 2 : kMost;
+      const int* own = total + bins - ((int)threadIdx.x + 1) * each;  // the lowest of them
+      int mine[kMost], sum = 0;
+#pragma unroll
+      for (int x = 0; x < kMost; ++x) {
+        mine[x] = x < each ? own[x] : 0;
+        sum += mine[x];
+      }
+      int all, above = cta_scan<W>(sum, buf[d & 1], &all);
+      if (above < room && above + sum >= room) {  // one thread
+#pragma unroll
+        for (int x = kMost - 1; x >= 0; --x) {
+          if (x < each && above < room && above + mine[x] >= room) {
+            s_bin = bins - ((int)threadIdx.x + 1) * each + x;
+            s_above = above;
+            s_in = mine[x];
+            above = room;  // found
+          } else {
+            above += mine[x];
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= (uint32_t)s_bin << shift;
+      known |= (uint32_t)(bins - 1) << shift;
+      room -= s_above;
+      exact = s_in == room;
+      if (exact) break;  // the same in every CTA
+      join();            // s_bin, its neighbours and the sums are read
+    }
+    threshold = prefix;
   }
+
+  // Ranks in row order: per group a count, then its sum over the groups before, over
+  // the CTA (each thread has some consecutive groups) and the cluster's CTAs before.
+  const int groups = W * steps, per_thread = (groups + W * 32 - 1) / (W * 32);
+  auto ranks = [&](int* at, auto count_of, int slot) {
+    const int g0 = threadIdx.x * per_thread;
+    int mine = 0, all;
+    for (int g = g0; g < g0 + per_thread && g < groups; ++g) mine += count_of(g);
+    int before = cta_scan<W>(mine, buf[slot & 1], &all);
+    if (threadIdx.x == 0) s_totals[slot] = all;
+    join();
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < rank) before += *cluster.map_shared_rank(&s_totals[slot], c);
+    for (int g = g0; g < g0 + per_thread && g < groups; ++g) {
+      const int n_g = count_of(g);  // (the counts may lie where the ranks go)
+      at[g] = before;
+      before += n_g;
+    }
+  };
+  if (!exact) {  // all digits known: keys equal to the threshold, in row order
+#pragma unroll
+    for (int i = 0; i < steps; ++i) {
+      const uint32_t same = __ballot_sync(kAll, row_of(i) < n && key(i) == threshold);
+      if (lane == 0) hole_at[i * W + warp] = __popc(same);
+    }
+    __syncthreads();
+    ranks(hole_at, [&](int g) { return hole_at[g]; }, 0);
+    __syncthreads();
+  }
+
+  // per 32 rows the mask of those that stay
+#pragma unroll
+  for (int i = 0; i < steps; ++i) {
+    const int row = row_of(i);
+    const uint32_t k = n > budget ? key(i) : 0;
+    uint32_t mask;
+    if (exact) {
+      mask = __ballot_sync(kAll, row < n && k >= threshold);
+    } else {
+      const uint32_t same = __ballot_sync(kAll, row < n && k == threshold);
+      const int before = hole_at[i * W + warp] + __popc(same & ((1u << lane) - 1));
+      mask = __ballot_sync(kAll, row < n && (k > threshold || (k == threshold && before < room)));
+    }
+    if (lane == 0) masks[i * W + warp] = mask;
+  }
+  // the bits of group g that are places
+  auto places = [&](int g) -> uint32_t {
+    const int x = kept - (cta_row + 32 * g);
+    return x >= 32 ? kAll : (x <= 0 ? 0u : (1u << x) - 1);
+  };
+  __syncthreads();
+  if (n > budget) {
+    ranks(hole_at, [&](int g) { return __popc(~masks[g] & places(g)); }, 1);
+    ranks(move_at, [&](int g) { return __popc(masks[g] & ~places(g)); }, 2);
+    __syncthreads();
+    int* list = count == 1 ? freed : cluster.map_shared_rank(freed, 0);
+    for (int g = warp; g < groups && places(g) != 0; g += W) {
+      const uint32_t out = ~masks[g] & places(g);
+      if (out >> lane & 1u) list[hole_at[g] + __popc(out & ((1u << lane) - 1))] = cta_row + 32 * g + lane;
+    }
+    // The list is complete; and, in place, every CTA has read its keys.
+    join();
+  }
+
+  // Copies: each warp its rows that stay (in place: that move).  They are listed until
+  // the list could overflow, so that many rows' reads are in flight at once.
+  const int per_pass = 32 / lanes, part = lane / lanes;
+  constexpr int kAhead = 4;
+  int listed = 0;
+  for (int i = 0; i < steps; ++i) {
+    const int g = i * W + warp, first = cta_row + 32 * g;
+    const uint32_t low = places(g), mask = masks[g], moving = mask & ~low, todo = a.in_place ? moving : mask;
+    if (todo >> lane & 1u) {
+      const int at = move_at[g] + __popc(moving & ((1u << lane) - 1));
+      const int to = low >> lane & 1u ? first + lane : (count == 1 ? freed[at] : *cluster.map_shared_rank(freed + at, 0));
+      s_copy[warp][listed + __popc(todo & ((1u << lane) - 1))] = make_int2(first + lane, to);
+    }
+    listed += __popc(todo);
+    if (listed <= kListed - 32 && i + 1 < steps) continue;
+    __syncwarp();
+    for (int r = lane; r < listed; r += 32) {
+      const int2 c = s_copy[warp][r];
+      const float w = weights[c.x];
+      const int at = positions[c.x];
+      a.to.weights[to0 + c.y] = w;
+      a.to.positions[to0 + c.y] = at;
+    }
+    for (int r0 = part; r0 < listed; r0 += kAhead * per_pass) {
+      uint4 code[kAhead];
+      uint32_t scale[kAhead];
+      int to[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int r = r0 + x * per_pass;
+        const int2 c = s_copy[warp][r < listed ? r : 0];
+        to[x] = r < listed && works ? c.y : -1;
+        if (works) {  // past the last row: the first once more
+          code[x] = code_from[(int64_t)c.x * p];
+          scale[x] = scale_from[(int64_t)c.x * p];
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x)
+        if (to[x] >= 0) {
+          code_to[(int64_t)to[x] * p] = code[x];
+          scale_to[(int64_t)to[x] * p] = scale[x];
+        }
+    }
+    __syncwarp();
+    listed = 0;
+  }
+  if (count > 1) cluster.sync();  // the list is read: its CTA may leave
 }
 
 template <int W, int K>
-cudaError_t launch(const EvictArgs& a, int64_t batch, int64_t n, int shares, cudaStream_t s) {
-  const size_t smem = evict_shared(n, a.budget);
+cudaError_t launch(const EvictArgs& a, int64_t batch, int64_t n, int count, cudaStream_t s) {
+  const int64_t steps = K > 0 ? K : (n + (int64_t)count * W * 32 - 1) / ((int64_t)count * W * 32);
+  const size_t smem = evict_shared(W * steps, evict_moves(n, a.budget));
   // the size varies from call to call: allow the largest that kv4_evict_fits lets through
-  const cudaError_t e = smem <= 48 * 1024 ? cudaSuccess : allow_shared<kv4_evict_kernel<W, K>>(kSharedMost);
+  const cudaError_t e = allow_shared<kv4_evict_kernel<W, K>>(kSharedMost);
   if (e != cudaSuccess) return e;
-  const int64_t grid = batch * a.kv_heads * shares;
+  const int64_t grid = batch * a.kv_heads * count;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  return launch_cluster(kv4_evict_kernel<W, K>, grid, W * 32, smem, shares, s, a, shares, (int)evict_moves(n, a.budget));
+  return launch_cluster(kv4_evict_kernel<W, K>, grid, W * 32, smem, count, s, a, count, (int)steps);
 }
 
 }  // namespace
 
-bool kv4_evict_fits(int64_t n, int64_t budget) { return evict_shared(n, budget) <= kSharedMost; }
+bool kv4_evict_fits(int64_t n, int64_t budget) {
+  return evict_shared(n / 32 + 1024, evict_moves(n, budget)) <= kSharedMost;  // groups: of one CTA at most
+}
 
 cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_place, int64_t batch, int64_t kv_heads,
                              int64_t head_dim, int64_t length, const int* lengths, int64_t budget,
@@ -296,13 +409,14 @@ cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_pla
   a.code_pieces = (int)(head_dim / 32);
   a.in_place = in_place;
   const int64_t n = lengths ? from.cache_len : (length < from.cache_len ? length : from.cache_len);
-  // CTAs per head that share the moves: at least 256 places each, while the heads leave SMs idle
-  int shares = 1;
-  while (shares < 8 && batch * kv_heads * shares * 2 <= 2 * device_sm_count() && budget >= 256 * shares * 2) shares *= 2;
-  if (n <= 8 * 256) return launch<8, 8>(a, batch, n, shares, s);
-  if (n <= 8 * 1024) return launch<32, 8>(a, batch, n, shares, s);
-  if (n <= 32 * 1024) return launch<32, 32>(a, batch, n, shares, s);
-  return launch<32, 0>(a, batch, n, shares, s);
+  // CTAs per head: while they leave room on the GPU (2 of 512 threads per SM) and have 2048 rows each
+  int count = 1;
+  while (count < 8 && batch * kv_heads * count * 2 <= 2 * device_sm_count() && n >= 2048 * count * 2) count *= 2;
+  const int64_t mine = (n + count - 1) / count;
+  if (mine <= 8 * 256) return launch<8, 8>(a, batch, n, count, s);
+  if (mine <= 8 * 512) return launch<16, 8>(a, batch, n, count, s);
+  if (mine <= 16 * 512) return launch<16, 16>(a, batch, n, count, s);
+  return launch<16, 0>(a, batch, n, count, s);
 }
 
 }  // namespace hrm

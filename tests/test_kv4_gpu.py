@@ -473,3 +473,14 @@ def test_long_caches_nan_rows_and_lse_order(cuda):
         nan = torch.isnan(got[0, -1])
         want = torch.zeros_like(nan); want[:, 32:64] = True
         assert torch.equal(nan, want)
+
+
+@pytest.mark.parametrize("n,budget", [(5000, 1111), (9000, 100), (20000, 19000), (70000, 30000), (140000, 700)])
+def test_evict_equal_weights_over_several_ctas(cuda, n, budget):
+    """All keys equal, and a few distinct values: thresholds that many rows share."""
+    c = filled(1, 2, n, 64, 17)
+    c.weights[0, 0] = 0.25
+    c.weights[0, 1] = torch.arange(n, device="cuda").remainder(5).float() * 1e-3
+    out = ops.kv4_cache(1, 2, budget, 64, track=True)
+    check_evict(c, n, budget, n - 10, out, host=True)
+    check_evict(c, n, budget, n - 10, host=True)
