@@ -47,7 +47,11 @@ struct Pre {
   static constexpr int kN = tile_rows<D>();  // cache rows of a tile
   static constexpr int kGroups = D / kKv4Group;
   static constexpr int kSoftmax = NQ * 128, kFill = 128;
-  static constexpr int kThreads = kSoftmax + kFill;
+  static constexpr int kThreads = kSoftmax + kFill + (NQ == 2 ? 128 : 32);
+  // NQ = 2: 4 warps on each scheduler would leave a thread 128 registers, too few for
+  // a row of 128 scores.  The warpgroups share the launch's registers out again.
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kFillRegs = 104, kMmaRegs = 72;
+  static_assert(NQ == 1 || 2 * kSoftmaxRegs + kFillRegs + kMmaRegs <= 4 * kLaunchRegs);
   static constexpr int kQ = 0, kQBytes = kM * D * 2;              // per query tile
   static constexpr int kK = NQ * kQBytes, kKBytes = kN * D * 2;   // per stage
   static constexpr int kV = kK + 2 * kKBytes, kVBytes = D * kN * 2;
@@ -56,7 +60,7 @@ struct Pre {
 };
 
 // Barriers, in order.
-enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kOFull = 12, kBars = 14 };
+enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPHalf = 10, kPFull = 12, kOFull = 14, kBars = 16 };
 
 struct PrefillSplit {
   int count;     // CTAs per item (kv head x block of query rows)
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
   auto bar = [&](int i) -> uint32_t { return bar0 + 8 * i; };
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   grid_dependency_begin();
 
   const unsigned rows = a.group * a.seq;
@@ -221,10 +225,11 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(bar(kKFull + i), T::kFill);
-        mbar_init(bar(kKEmpty + i), NQ);
+        mbar_init(bar(kKEmpty + i), 1);
         mbar_init(bar(kVFull + i), T::kFill);
-        mbar_init(bar(kVEmpty + i), NQ);
+        mbar_init(bar(kVEmpty + i), 1);
         mbar_init(bar(kSFull + i), 1);
+        mbar_init(bar(kPHalf + i), kM);
         mbar_init(bar(kPFull + i), kM);
         mbar_init(bar(kOFull + i), 1);
       }
@@ -252,6 +257,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
 
   if (warp < T::kSoftmax / 32) {
     // ---------------------------------------------------------------- softmax
+    if (NQ == 2) take_registers<T::kSoftmaxRegs>();
     const int qt = warp / 4, r = qt * kM + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + qt * kN, o_at = tmem + lanes + NQ * kN + qt * D;
@@ -260,22 +266,6 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     float m = -INFINITY, l = 0.0f;  // m: of the unscaled scores, as of the last rescale
     uint32_t bad = 0;  // bit g: group g of v
     bool ok = true;
-    // Products, by the tile's first thread.  They run in the order of their issue.
-    const bool issuer = (warp & 3) == 0 && lane == 0;
-    constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
-    auto scores = [&](int j) {  // S of tile j; false if its keys do not come
-      if (!mbar_wait_bounded(bar(kKFull + (j & 1)), (j >> 1) & 1)) return;
-      tcgen05_after_sync();
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        tcgen05_mma(tmem + qt * kN, panel_desc(base + T::kQ + qt * T::kQBytes + (k / 4) * (kM * 128) + 32 * (k % 4)),
-                    panel_desc(base + T::kK + (j & 1) * T::kKBytes + (k / 4) * (kN * 128) + 32 * (k % 4)), kShapeS,
-                    k > 0);
-      tcgen05_commit(bar(kSFull + qt));
-      tcgen05_commit(bar(kKEmpty + (j & 1)));
-    };
-    if (issuer && n > 0) scores(0);
-    __syncwarp();
     for (int j = 0; j < n; ++j) {
       const int first = (j0 + j) * kN;
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kSFull + qt), j & 1));
@@ -323,6 +313,25 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
           }
         }
       }
+      if (first + kN > lowest && lowest < limit) {
+        // rows that some query must not see: the groups of v that are not finite were read
+        // as zeros (before P is handed over: the products free the flags' buffer)
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1));
+        if (!ok) break;
+        const uint2* flags = reinterpret_cast<const uint2*>(s_bad[j & 1]);
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < kN / 32; ++i) any |= flags[32 * i + lane].x | flags[32 * i + lane].y;
+        if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll 1
+          for (int i = 0; i < kN && first + i < lim; ++i) {
+            const uint2 f = flags[i];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) bad |= (f.x >> (8 * x) & 1u) << x | (f.y >> (8 * x) & 1u) << (4 + x);
+          }
+          __syncwarp();
+        }
+      }
       const float shift = m == -INFINITY ? 0.0f : m * scale;
       const uint64_t scale2 = pack_f32x2(__float_as_uint(scale), __float_as_uint(scale));
       const uint64_t shift2 = pack_f32x2(__float_as_uint(-shift), __float_as_uint(-shift));
@@ -338,40 +347,14 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
           p[i] = pack_bf16x2(p0, p1);
         }
         tmem_store16(s_at + 16 * c, p);  // over scores that this thread has in registers
+        if (c + 1 == kN / 64 || c + 1 == kN / 32) {
+          tmem_wait_store();
+          tcgen05_before_sync();
+          mbar_arrive(bar((c + 1 == kN / 64 ? kPHalf : kPFull) + qt));
+        }
       }
-      tmem_wait_store();
-      tcgen05_before_sync();
-      mbar_arrive(bar(kPFull + qt));
       const uint64_t both = add_f32x2(sum[0], sum[1]);
       l += lo_f32(both) + hi_f32(both);
-      if (issuer && mbar_wait_bounded(bar(kPFull + qt), j & 1) &&
-          mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1)) {
-        tcgen05_after_sync();
-#pragma unroll
-        for (int k = 0; k < kN / 16; ++k)
-          tcgen05_mma_ta(tmem + NQ * kN + qt * D, tmem + qt * kN + 8 * k,
-                         panel_desc(base + T::kV + (j & 1) * T::kVBytes + (k / 4) * (D * 128) + 32 * (k % 4)), kShapeO,
-                         j > 0 || k > 0);
-        tcgen05_commit(bar(kVEmpty + (j & 1)));
-        if (j + 1 < n)
-          scores(j + 1);  // replaces P, which the products before it have read by then
-        else
-          tcgen05_commit(bar(kOFull + qt));
-      }
-      __syncwarp();
-      if (first + kN > lowest && lowest < limit) {
-        // rows that some query must not see: the groups of v that are not finite were read as zeros
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1));
-        if (!ok) break;
-        const uint2* flags = reinterpret_cast<const uint2*>(s_bad[j & 1]);
-        for (int i = 0; i < kN && first + i < lim; ++i) {
-          const uint2 f = flags[i];
-          if ((f.x | f.y) == 0) continue;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) bad |= (f.x >> (8 * x) & 1u) << x | (f.y >> (8 * x) & 1u) << (4 + x);
-        }
-        __syncwarp();
-      }
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kOFull + qt), 0));
     tcgen05_after_sync();
@@ -427,8 +410,9 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       tail[NQ * kM] = l;
       tail[2 * NQ * kM] = __uint_as_float(bad);
     }
-  } else {
+  } else if (warp < (T::kSoftmax + T::kFill) / 32) {
     // --------------------------------------------------------------- filling
+    if (NQ == 2) give_registers<T::kFillRegs>();
     const int t = tid - T::kSoftmax;
     const int64_t head_row = (int64_t)bh * a.c.cache_len;
     const uint8_t* kc = a.c.k_codes + head_row * (D / 2);
@@ -453,6 +437,54 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(bar(kVFull + s));
       if (j + 1 < n) c.fetch_v(vc, vs, first + kN, limit, t);
+    }
+  } else {
+    // -------------------------------------------------------------- products
+    // By one thread; they run in the order of their issue.
+    if (NQ == 2) give_registers<T::kMmaRegs>();
+    if (warp == (T::kSoftmax + T::kFill) / 32 && elect_one()) {
+      constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
+      auto scores = [&](int qt, int s) {  // of the keys of stage s
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tcgen05_mma(tmem + qt * kN, panel_desc(base + T::kQ + qt * T::kQBytes + (k / 4) * (kM * 128) + 32 * (k % 4)),
+                      panel_desc(base + T::kK + s * T::kKBytes + (k / 4) * (kN * 128) + 32 * (k % 4)), kShapeS, k > 0);
+        tcgen05_commit(bar(kSFull + qt));
+      };
+      bool run = n > 0 && mbar_wait_bounded(bar(kKFull), 0);
+      if (run) {
+        tcgen05_after_sync();
+#pragma unroll
+        for (int qt = 0; qt < NQ; ++qt) scores(qt, 0);
+        tcgen05_commit(bar(kKEmpty));
+      }
+      for (int j = 0; j < n && run; ++j) {
+        const int s = j & 1, phase = (j >> 1) & 1;
+        run = mbar_wait_bounded(bar(kVFull + s), phase);
+        if (j + 1 < n) run = run && mbar_wait_bounded(bar(kKFull + (s ^ 1)), ((j + 1) >> 1) & 1);
+#pragma unroll
+        for (int qt = 0; qt < NQ; ++qt) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            run = run && mbar_wait_bounded(bar((half == 0 ? kPHalf : kPFull) + qt), j & 1);
+            if (!run) break;
+            tcgen05_after_sync();
+#pragma unroll
+            for (int k = half * (kN / 32); k < (half + 1) * (kN / 32); ++k)
+              tcgen05_mma_ta(tmem + NQ * kN + qt * D, tmem + qt * kN + 8 * k,
+                             panel_desc(base + T::kV + s * T::kVBytes + (k / 4) * (D * 128) + 32 * (k % 4)), kShapeO,
+                             j > 0 || k > 0);
+          }
+          if (!run) break;
+          if (qt == NQ - 1) tcgen05_commit(bar(kVEmpty + s));
+          if (j + 1 < n) {
+            scores(qt, s ^ 1);  // replace P, which the products before them have read by then
+            if (qt == NQ - 1) tcgen05_commit(bar(kKEmpty + (s ^ 1)));
+          } else {
+            tcgen05_commit(bar(kOFull + qt));
+          }
+        }
+      }
     }
   }
   __syncwarp();
@@ -575,7 +607,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
   auto bar = [&](int i) -> uint32_t { return bar0 + 8 * i; };
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   grid_dependency_begin();
   const unsigned rows = a.group * a.seq;
   const int bh = (int)(blockIdx.x / (unsigned)tiles_k), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
@@ -698,7 +730,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
       fence_proxy_async_smem();
       mbar_arrive(bar(kWFull + s));
     }
-  } else if (lane == 0) {
+  } else if (elect_one()) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t kShape = mma_shape(128, 128);
     int n = 0;
@@ -753,6 +785,7 @@ cudaError_t launch_prefill(const AttnArgs& a, const PrefillShape& p, int64_t lon
   while (p.items * (split.count + 1) <= device_sm_count() && (split.count + 1) * 4 * T::kN <= longest) ++split.count;
   if (p.items * split.count > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaError_t e = allow_shared<kv4_prefill_kernel<D, NQ>>(T::kSmem);
+  if (e == cudaSuccess && NQ == 2) e = has_registers<kv4_prefill_kernel<D, NQ>>(T::kLaunchRegs);
   if (e != cudaSuccess) return e;
   e = launch_kernel(kv4_prefill_kernel<D, NQ>, p.items * split.count, T::kThreads, T::kSmem, s, a, split, p.blocks_q);
   if (e != cudaSuccess || split.count == 1) return e;

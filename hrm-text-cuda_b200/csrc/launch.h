@@ -89,6 +89,21 @@ inline cudaError_t allow_shared(size_t bytes) {
   return e;
 }
 
+// For a kernel whose warpgroups share its registers out again: whether it was built
+// with `regs` per thread.  With fewer the taking would wait for good.
+template <auto K>
+inline cudaError_t has_registers(int regs) {
+  static std::atomic<int> built{0};
+  int n = built.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, K);
+    if (e != cudaSuccess) return e;
+    built.store(n = attr.numRegs, std::memory_order_relaxed);
+  }
+  return n >= regs ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+
 cudaError_t launch_additive_inject(const void* a, const void* b, void* out, int64_t n, cudaStream_t s);
 cudaError_t launch_attn_gate(const void* gate, const void* attn, void* out, int64_t n, cudaStream_t s);
 cudaError_t launch_broadcast(void* dst, const void* src, int64_t n_copies, int64_t vec_len, cudaStream_t s);

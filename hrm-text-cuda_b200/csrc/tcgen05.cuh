@@ -23,6 +23,14 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
   return true;
 }
 
+// Registers of a thread from here on, by all threads of a warpgroup: `take` waits until
+// others have given them up.  The launch's registers (those of the kernel, for all its
+// threads) have to cover what the warpgroups ask for in the end.
+template <int N>
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
 // ------------------------------------------------------------ tensor memory
 // One warp allocates and frees; the address is written to shared memory.
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t columns) {
@@ -95,6 +103,14 @@ __device__ __forceinline__ uint64_t panel_desc(uint32_t addr) {
 // Instruction descriptor: bf16 x bf16 -> fp32, M x N, both operands K-major.
 __host__ __device__ constexpr uint32_t mma_shape(int m, int n) {
   return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
+}
+// True for one thread of a warp that is here together.  The compiler knows of this form
+// that one thread follows and that the values it uses are the warp's: products issued
+// under a test of the lane number took twice as long to issue (119 cycles each).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
 }
 // D (tensor memory) = A * B^T [+ D], K = 16; issued by one thread.
 __device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {

@@ -35,6 +35,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _launch(name: str, device: torch.device, tensors, stream: Optional[torch.cuda.Stream], *args) -> None:
     """ops._launch for calls of a few microseconds: the same checks (every tensor and
     an explicit stream on `device`, which is current during the call), on plain
@@ -48,7 +51,7 @@ def _launch(name: str, device: torch.device, tensors, stream: Optional[torch.cud
         raise ValueError(f"{name}: stream on {stream.device} but tensors on {device}")
     else:
         handle = stream.cuda_stream
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         status = getattr(LIB, name)(*args, handle)
     else:
         with torch.cuda.device(device):
@@ -164,15 +167,18 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
     s = gqkv.shape[1]
     if out is None:
-        new = gqkv.new_empty
-        kv = (b, h, s, d)
-        out = (new((b, s, h, d)), new(kv), new(kv) if keep_kv else None, new(kv) if keep_kv else None)
-    for t, n in zip(out, ("gate", "q", "k", "v")):
-        if t is None and n in ("k", "v"):
-            continue
-        _need(t, n)
-        if t.numel() != b * s * h * d:
-            raise ValueError(f"{n} has the wrong size")
+        new, kv = gqkv.new_empty, (b, h, s, d)
+        gate, q = new((b, s, h, d)), new(kv)
+        k, v = (new(kv), new(kv)) if keep_kv else (None, None)
+        given = ()
+    else:
+        gate, q, k, v = given = tuple(out)
+        for t, n in zip(given, ("gate", "q", "k", "v")):
+            if t is None and n in ("k", "v"):
+                continue
+            _need(t, n)
+            if t.numel() != b * s * h * d:
+                raise ValueError(f"{n} has the wrong size")
     positions = 0
     if table is not None:
         _need(table, "table", (torch.float32,))
@@ -181,9 +187,10 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         positions = table.shape[0]
     pos, pos_t = _offset(position_offset, "position_offset", b)
     off, off_t = _offset(cache_offset, "cache_offset", b)
-    _launch("hrm_split_gqkv_rope_kv4", cache.device, (gqkv, *out, table, pos_t, off_t), stream, _ptr(gqkv),
-            *(_ptr(t) for t in out), cache._ref, s, pos, _ptr(pos_t), theta, _ptr(table), positions, off, _ptr(off_t))
-    return tuple(out)
+    _launch("hrm_split_gqkv_rope_kv4", cache.device, (gqkv, table, pos_t, off_t, *given), stream, gqkv.data_ptr(),
+            gate.data_ptr(), q.data_ptr(), _ptr(k), _ptr(v), cache._ref, s, pos, _ptr(pos_t), theta, _ptr(table),
+            positions, off, _ptr(off_t))
+    return gate, q, k, v
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gate: Optional[torch.Tensor] = None,
