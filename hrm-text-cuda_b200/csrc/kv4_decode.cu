@@ -246,7 +246,7 @@ __device__ __forceinline__ void v_step_one(float (*o)[4], const uint32_t (&a)[2]
            fma_bf16x2(kv4_pair<P>(a[1]), s2[1], z2[1]), fma_bf16x2(kv4_pair<P>(b[1]), s2[1], z2[1]), p[0], p[1]);
 }
 
-__device__ __forceinline__ float sigmoid_gate(uint16_t g) { return 1.0f / (1.0f + __expf(-bf16_to_f32(g))); }
+__device__ __forceinline__ float sigmoid_gate(uint16_t g) { return gate_factor(bf16_to_f32(g)); }
 
 // Writes elements d, d + 1 of query row r of the item: gated, rounded once.
 __device__ __forceinline__ int64_t out_at(const AttnArgs& a, const Item& x, int64_t head_dim, int r, int d) {

@@ -10,6 +10,14 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2^x, within 2 ulp; 0
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// sigmoid(g), what the gate of an output multiplies it by, within 4 ulp of fp32: far
+// below the rounding of the bf16 product.  (The exact division is a call of some 40
+// instructions; in a prompt's 128 x 256 outputs per CTA it took as long as 4 tiles.)
+__device__ __forceinline__ float gate_factor(float g) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + __expf(-g)));
+  return y;
+}
 // D = A (16x16, row) * B (16x8, col) + D, bf16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -58,15 +66,21 @@ struct AttnArgs {
   float* lse;     // weights wanted, more rows: [batch, heads, seq], log2 of each row's sum of 2^score
 };
 
-// Cache rows that query s of sequence b sees: [0, limit).
-__device__ __forceinline__ int visible_rows(const AttnArgs& a, int b, int s) {
-  const int64_t off = a.cache_offsets ? a.cache_offsets[b] : a.cache_offset;
-  int64_t lim = off + s + 1;
-  if (lim < a.prefix_len) lim = a.prefix_len;
-  if (lim > off + a.seq) lim = off + a.seq;
-  if (lim > a.c.cache_len) lim = a.c.cache_len;
-  return lim < 0 ? 0 : (int)lim;
-}
+// Cache rows that the queries of a sequence see: query s rows [0, rows(s)).
+struct Visible {
+  int64_t off, prefix, top;
+  __device__ __forceinline__ Visible(const AttnArgs& a, int b)
+      : off(a.cache_offsets ? a.cache_offsets[b] : a.cache_offset), prefix(a.prefix_len) {
+    top = off + a.seq < a.c.cache_len ? off + a.seq : a.c.cache_len;
+  }
+  __device__ __forceinline__ int rows(int s) const {
+    int64_t lim = off + s + 1;
+    if (lim < prefix) lim = prefix;
+    if (lim > top) lim = top;
+    return lim < 0 ? 0 : (int)lim;
+  }
+};
+__device__ __forceinline__ int visible_rows(const AttnArgs& a, int b, int s) { return Visible(a, b).rows(s); }
 
 // A word (S, Z) whose group reads back as NaN or an infinity.
 __device__ __forceinline__ bool kv4_not_finite(uint32_t sz) {

@@ -49,8 +49,9 @@ struct Pre {
   static constexpr int kSoftmax = NQ * 128, kFill = 128;
   static constexpr int kThreads = kSoftmax + kFill + (NQ == 2 ? 128 : 32);
   // NQ = 2: 4 warps on each scheduler would leave a thread 128 registers, too few for
-  // a row of 128 scores.  The warpgroups share the launch's registers out again.
-  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kFillRegs = 104, kMmaRegs = 72;
+  // a row of 128 scores.  The warpgroups share the launch's registers out again
+  // (chunk of 512 over 8192: 51 us; 168 + 104 + 72: 60; 152 + 120 + 88: 60).
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kFillRegs = 120, kMmaRegs = 72;
   static_assert(NQ == 1 || 2 * kSoftmaxRegs + kFillRegs + kMmaRegs <= 4 * kLaunchRegs);
   static constexpr int kQ = 0, kQBytes = kM * D * 2;              // per query tile
   static constexpr int kK = NQ * kQBytes, kKBytes = kN * D * 2;   // per stage
@@ -72,6 +73,15 @@ __host__ __device__ inline int64_t prefill_part(int nq, int64_t head_dim) { retu
 __device__ __forceinline__ uint4 paired_order(const uint4& v) {
   return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                     __byte_perm(v.y, v.w, 0x7632));
+}
+
+// Query rows [r0, + count) of a kv head: the highest and the lowest number of cache
+// rows that one of them sees (rows past the last: none).
+__device__ __forceinline__ int2 row_limits(const Visible& see, unsigned seq, unsigned rows, unsigned r0, unsigned count) {
+  const unsigned r1 = min(r0 + count, rows) - 1;
+  const unsigned g0 = r0 / seq, s0 = r0 - g0 * seq, g1 = r1 / seq, s1 = r1 - g1 * seq;
+  return make_int2(see.rows((int)(g0 == g1 ? s1 : seq - 1)),
+                   r0 + count > rows ? 0 : see.rows((int)(g0 == g1 ? s0 : 0)));
 }
 
 // A filling thread's share of a tile of N rows: pieces (16 bytes of codes, one group)
@@ -173,7 +183,6 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kBars];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_limit[NQ * kM];
   __shared__ __align__(16) uint8_t s_bad[2][kN][8];  // per stage and cache row: groups of v that are not finite
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
@@ -193,10 +202,6 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   auto q_row0 = [&]() -> int64_t { return ((int64_t)b * a.heads + hk * a.group) * a.seq; };
 
   // ---- set-up: limits, queries, barriers, tensor memory
-  for (int r = tid; r < NQ * kM; r += T::kThreads) {
-    const unsigned row = row0 + r;
-    s_limit[r] = row < rows ? visible_rows(a, b, row % a.seq) : -1;
-  }
   {
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;  // the softmax takes |scale|
     const uint32_t keep = a.scale_log2 == 0.0f ? 0u : 0xffffffffu;  // scale 0: all scores 0
@@ -220,6 +225,18 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       }
     }
   }
+  const Visible see(a, b);
+  const int2 limits = row_limits(see, a.seq, rows, row0, NQ * kM);
+  const int limit = limits.x, lowest = limits.y;
+  const int tiles = (limit + kN - 1) / kN;
+  int j0 = 0, j1 = tiles;
+  if (split.count > 1) {
+    j0 = (int)((int64_t)tiles * rank / split.count);
+    j1 = (int)((int64_t)tiles * (rank + 1) / split.count);
+  }
+  const int n = j1 - j0;
+  constexpr int kFillFirst = T::kSoftmax / 32, kMmaWarp = kFillFirst + T::kFill / 32;
+  const bool fills = warp >= kFillFirst && warp < kMmaWarp;
   for (int i = tid; i < 2 * kN; i += T::kThreads) *reinterpret_cast<uint2*>(s_bad[i / kN][i % kN]) = make_uint2(0, 0);
   if (warp == 0) {
     if (lane == 0) {
@@ -244,24 +261,13 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   tcgen05_after_sync();
   const uint32_t tmem = s_tmem;
 
-  int limit = 0, lowest = INT32_MAX;
-  for (int r = lane; r < NQ * kM; r += 32) {
-    limit = max(limit, s_limit[r]);
-    if (s_limit[r] >= 0) lowest = min(lowest, s_limit[r]);
-  }
-  limit = __reduce_max_sync(0xffffffffu, limit);
-  lowest = __reduce_min_sync(0xffffffffu, lowest);
-  const int tiles = (limit + kN - 1) / kN;
-  const int j0 = (int)((int64_t)tiles * rank / split.count), j1 = (int)((int64_t)tiles * (rank + 1) / split.count);
-  const int n = j1 - j0;
-
-  if (warp < T::kSoftmax / 32) {
+  if (warp < kFillFirst) {
     // ---------------------------------------------------------------- softmax
     if (NQ == 2) take_registers<T::kSoftmaxRegs>();
     const int qt = warp / 4, r = qt * kM + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + qt * kN, o_at = tmem + lanes + NQ * kN + qt * D;
-    const int lim = s_limit[r];
+    const int lim = row0 + r < rows ? see.rows((int)((row0 + r) % a.seq)) : -1;
     const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
     float m = -INFINITY, l = 0.0f;  // m: of the unscaled scores, as of the last rescale
     uint32_t bad = 0;  // bit g: group g of v
@@ -356,16 +362,38 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       const uint64_t both = add_f32x2(sum[0], sum[1]);
       l += lo_f32(both) + hi_f32(both);
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kOFull + qt), 0));
-    tcgen05_after_sync();
     const unsigned row = row0 + r;
     const unsigned g = row / a.seq, sq = row - g * a.seq;
     const int64_t head = hk * a.group + g;
+    const int64_t out_at = row < rows ? (((int64_t)b * a.seq + sq) * a.heads + head) * D : -1;
+    // A thread has a row, but 32 rows' pieces of 16 bytes lie 32 heads' rows apart: gate
+    // and output pass through the warp's 32 rows of the query tile, free since the last S,
+    // so that a warp's access covers whole rows.  (Accesses by row took 28000 cycles
+    // for 256 rows of 128 elements with a gate, as long as 8 tiles.)
+    uint8_t* const mine = smem + T::kQ + qt * T::kQBytes;
+    const int warp_row = (warp & 3) * 32;
+    auto each_piece = [&](auto&& f) {  // f(place in the output or -1, place in the tile)
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        const int x = 32 * i + lane, in_warp = x / (D / 8), p = x % (D / 8);
+        const int64_t at = __shfl_sync(0xffffffffu, out_at, in_warp);
+        f(at < 0 ? at : at + 8 * p, mine + (p / 8) * (kM * 128) + panel_piece(warp_row + in_warp, p % 8));
+      }
+    };
+    if (ok && split.count == 1 && a.gate != nullptr) {
+      each_piece([&](int64_t at, uint8_t* place) {
+        cp_async_zfill<16>(smem_addr(place), a.gate + (at < 0 ? 0 : at), at >= 0);
+      });
+      cp_async_commit();
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kOFull + qt), 0));
+    tcgen05_after_sync();
     if (split.count == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (row < rows && a.lse != nullptr)
         a.lse[q_row0() + row] = m == -INFINITY ? -INFINITY : m * scale + log2f(l);
-      const int64_t at = (((int64_t)b * a.seq + sq) * a.heads + head) * D;
+      cp_async_wait_all();
+      __syncwarp();
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -378,23 +406,29 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         }
         const bool nan = bad >> c & 1u;
 #pragma unroll
-        for (int i = 0; i < 4 && row < rows && ok; ++i) {
+        for (int i = 0; i < 4; ++i) {
+          const int p = 4 * c + i;
+          uint4* const place = reinterpret_cast<uint4*>(mine + (p / 8) * (kM * 128) + panel_piece(r % kM, p % 8));
           uint4 y, gate = make_uint4(0, 0, 0, 0);
-          if (a.gate != nullptr) gate = ld_l2(reinterpret_cast<const uint4*>(a.gate + at + 32 * c) + i);
+          if (a.gate != nullptr) gate = *place;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             float v0 = __uint_as_float(o[8 * i + 2 * w]) * inv, v1 = __uint_as_float(o[8 * i + 2 * w + 1]) * inv;
             if (nan) v0 = v1 = __int_as_float(0x7fc00000);
             if (a.gate != nullptr) {
-              v0 *= 1.0f / (1.0f + __expf(-bf16_lo(vget(gate, w))));
-              v1 *= 1.0f / (1.0f + __expf(-bf16_hi(vget(gate, w))));
+              v0 *= gate_factor(bf16_lo(vget(gate, w)));
+              v1 *= gate_factor(bf16_hi(vget(gate, w)));
             }
             vset(y, w, pack_bf16x2(v0, v1));
           }
-          st_l2(reinterpret_cast<uint4*>(a.out + at + 32 * c) + i, y);
+          *place = y;
         }
-        __syncwarp();
       }
+      __syncwarp();
+      if (ok)
+        each_piece([&](int64_t at, const uint8_t* place) {
+          if (at >= 0) st_l2(reinterpret_cast<uint4*>(a.out + at), *reinterpret_cast<const uint4*>(place));
+        });
     } else {
       float* part = split.parts + (int64_t)blockIdx.x * prefill_part(NQ, D);
 #pragma unroll 1
@@ -410,7 +444,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       tail[NQ * kM] = l;
       tail[2 * NQ * kM] = __uint_as_float(bad);
     }
-  } else if (warp < (T::kSoftmax + T::kFill) / 32) {
+  } else if (fills) {
     // --------------------------------------------------------------- filling
     if (NQ == 2) give_registers<T::kFillRegs>();
     const int t = tid - T::kSoftmax;
@@ -442,7 +476,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     // -------------------------------------------------------------- products
     // By one thread; they run in the order of their issue.
     if (NQ == 2) give_registers<T::kMmaRegs>();
-    if (warp == (T::kSoftmax + T::kFill) / 32 && elect_one()) {
+    if (warp == kMmaWarp && elect_one()) {
       constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
       auto scores = [&](int qt, int s) {  // of the keys of stage s
 #pragma unroll
@@ -561,8 +595,8 @@ __global__ void __launch_bounds__(kM) kv4_prefill_join_kernel(const AttnArgs a, 
       float v0 = sum[8 * i + 2 * w] * inv, v1 = sum[8 * i + 2 * w + 1] * inv;
       if (nan) v0 = v1 = __int_as_float(0x7fc00000);
       if (a.gate != nullptr) {
-        v0 *= 1.0f / (1.0f + __expf(-bf16_lo(vget(gate, w))));
-        v1 *= 1.0f / (1.0f + __expf(-bf16_hi(vget(gate, w))));
+        v0 *= gate_factor(bf16_lo(vget(gate, w)));
+        v1 *= gate_factor(bf16_hi(vget(gate, w)));
       }
       vset(y, w, pack_bf16x2(v0, v1));
     }
@@ -587,17 +621,38 @@ struct Wgt {
 };
 enum { kWFull = 0, kWEmpty = 2, kWSFull = 4, kWSEmpty = 6, kWBars = 8 };
 
-// Query rows [128 i, + 128) of a kv head: the highest and the lowest number of cache
-// rows that one of them sees (rows past the last: none).
-__device__ __forceinline__ int2 tile_limits(const AttnArgs& a, int b, unsigned rows, int i) {
-  const unsigned r0 = i * 128u, r1 = min(r0 + 127, rows - 1), seq = a.seq;
-  const unsigned g0 = r0 / seq, s0 = r0 - g0 * seq, g1 = r1 / seq, s1 = r1 - g1 * seq;
-  return make_int2(visible_rows(a, b, (int)(g0 == g1 ? s1 : seq - 1)),
-                   r0 + 127 >= rows ? 0 : visible_rows(a, b, (int)(g0 == g1 ? s0 : 0)));
-}
+// The query tiles of a kv head with a row that sees cache row `first` or one after it,
+// in order.  (Asking each tile in turn for its limits, divisions and all, took 750
+// cycles a tile.)
+struct QueryTiles {
+  const Visible see;
+  const unsigned seq, rows;
+  const int first;
+  unsigned row = 0, s = 0;  // the tile's first row, and which query of its head that is
+  int lowest = 0;           // cache rows that the one of its rows with the fewest sees
+  __device__ __forceinline__ QueryTiles(const Visible& see, unsigned seq, unsigned rows, int first)
+      : see(see), seq(seq), rows(rows), first(first) {}
+  __device__ __forceinline__ bool find() {  // from the present tile on; false past the last
+    while (row < rows) {
+      const bool more = s + 128 > seq;  // heads than one (or the end)
+      if (see.rows((int)(more ? seq - 1 : s + 127)) > first) {
+        lowest = row + 128 > rows ? 0 : see.rows((int)(more ? 0 : s));
+        return true;
+      }
+      // a head's last query sees `first`: on to the tile of the first query that does
+      step((unsigned)(first - see.off - s) / 128u);
+    }
+    return false;
+  }
+  __device__ __forceinline__ void step(unsigned tiles) {
+    row += 128 * tiles;
+    s += 128 * tiles;
+    if (s >= seq) s %= seq;
+  }
+};
 
 template <int D>
-__global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const AttnArgs a, const int tiles_k) {
+__global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const AttnArgs a) {
   using T = Wgt<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kWBars];
@@ -610,11 +665,13 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   grid_dependency_begin();
   const unsigned rows = a.group * a.seq;
-  const int bh = (int)(blockIdx.x / (unsigned)tiles_k), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
-  const int first = (int)(blockIdx.x - bh * tiles_k) * 128;
-  const int limit = visible_rows(a, b, a.seq - 1);  // of the last query: the highest
+  // all heads' first rows first: under a causal mask most queries see them
+  const unsigned heads_all = (unsigned)(a.batch * a.kv_heads), tile = blockIdx.x / heads_all;
+  const int bh = (int)(blockIdx.x - tile * heads_all), b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
+  const int first = (int)tile * 128;
+  const Visible see(a, b);
+  const int limit = see.rows(a.seq - 1);  // of the last query: the highest
   if (first >= limit) return;
-  const int tiles_q = (int)((rows + 127) / 128);
 
   const int64_t head_row = (int64_t)bh * a.c.cache_len;
   {  // the keys, elements in kv4_pair's order put back: the queries are copied as they are
@@ -663,14 +720,12 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     float extra = 0.0f;  // of tiles with masked probabilities
     const uint64_t scale2 = pack_f32x2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
     int n = 0;
-    for (int i = 0; i < tiles_q; ++i) {
-      const int2 see = tile_limits(a, b, rows, i);
-      if (see.x <= first) continue;
+    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
       const int s = n & 1, phase = (n >> 1) & 1, entry = n & 3;
       ++n;
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(kWSFull + s), phase))) break;
       tcgen05_after_sync();
-      const bool whole = first + 128 <= see.y;
+      const bool whole = first + 128 <= q.lowest;
       uint32_t x[2][32];  // 32 columns are loaded while the 32 before them are worked on
       tmem_load32(x[0], tmem + lanes + 128 * s);
 #pragma unroll
@@ -679,18 +734,18 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
         if (c < 3) tmem_load32(x[(c + 1) & 1], tmem + lanes + 128 * s + 32 * (c + 1));
         if (whole) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint4 lse = *reinterpret_cast<const uint4*>(&s_lse[entry][32 * c + 4 * q]);
-            const uint64_t y0 = fma_f32x2(pack_f32x2(x[c & 1][4 * q], x[c & 1][4 * q + 1]), scale2, pack_f32x2(lse.x, lse.y));
-            const uint64_t y1 = fma_f32x2(pack_f32x2(x[c & 1][4 * q + 2], x[c & 1][4 * q + 3]), scale2, pack_f32x2(lse.z, lse.w));
+          for (int i = 0; i < 8; ++i) {
+            const uint4 lse = *reinterpret_cast<const uint4*>(&s_lse[entry][32 * c + 4 * i]);
+            const uint64_t y0 = fma_f32x2(pack_f32x2(x[c & 1][4 * i], x[c & 1][4 * i + 1]), scale2, pack_f32x2(lse.x, lse.y));
+            const uint64_t y1 = fma_f32x2(pack_f32x2(x[c & 1][4 * i + 2], x[c & 1][4 * i + 3]), scale2, pack_f32x2(lse.z, lse.w));
             sum[0] = add_f32x2(sum[0], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y0))), __float_as_uint(exp2_approx(hi_f32(y0)))));
             sum[1] = add_f32x2(sum[1], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y1))), __float_as_uint(exp2_approx(hi_f32(y1)))));
           }
         } else {
 #pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (at < s_lim[entry][32 * c + q])
-              extra += exp2_approx(fmaf(__uint_as_float(x[c & 1][q]), a.scale_log2, s_lse[entry][32 * c + q]));
+          for (int i = 0; i < 32; ++i)
+            if (at < s_lim[entry][32 * c + i])
+              extra += exp2_approx(fmaf(__uint_as_float(x[c & 1][i]), a.scale_log2, s_lse[entry][32 * c + i]));
         }
       }
       tcgen05_before_sync();
@@ -703,28 +758,27 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     const int t = tid - 128;
     const int64_t q_row0 = ((int64_t)b * a.heads + hk * a.group) * a.seq;  // the head's query rows lie one after another
     const uint4* src = a.q + q_row0 * (D / 8);
-    auto fetch = [&](int i, int s) {
-      const int64_t at = (int64_t)i * (128 * (D / 8));
+    auto fetch = [&](unsigned row0, int s) {
+      const int64_t at = (int64_t)row0 * (D / 8);
 #pragma unroll
       for (int x = t; x < 128 * (D / 8); x += 128) {
         const int r = x / (D / 8), p = x % (D / 8);
-        const bool in = i * 128u + r < rows;
+        const bool in = row0 + r < rows;
         cp_async_zfill<16>(base + T::kQ + s * T::kBytes + (p / 8) * (128 * 128) + panel_piece(r, p % 8),
                            in ? src + at + x : src, in);
       }
     };
     int n = 0;
-    for (int i = 0; i < tiles_q; ++i) {
-      if (tile_limits(a, b, rows, i).x <= first) continue;
+    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
       const int s = n & 1, phase = (n >> 1) & 1;
       if (!mbar_wait_bounded(bar(kWEmpty + s), phase ^ 1)) break;
-      fetch(i, s);
+      fetch(q.row, s);
       cp_async_commit();
       // (entry n & 3 of lse and limits: its last reader freed the scores' buffer that the
       // products of tile n - 2, now done, went to)
-      const unsigned row = i * 128u + t;
+      const unsigned row = q.row + t, sq = q.s + t;
       s_lse[n & 3][t] = row < rows ? -a.lse[q_row0 + row] : 0.0f;
-      s_lim[n & 3][t] = row < rows ? visible_rows(a, b, (int)(row % (unsigned)a.seq)) : -1;
+      s_lim[n & 3][t] = row < rows ? see.rows((int)(sq < q.seq ? sq : sq % q.seq)) : -1;
       ++n;
       cp_async_wait_all();
       fence_proxy_async_smem();
@@ -734,8 +788,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     // ---------------------------------------------------------------- products
     constexpr uint32_t kShape = mma_shape(128, 128);
     int n = 0;
-    for (int i = 0; i < tiles_q; ++i) {
-      if (tile_limits(a, b, rows, i).x <= first) continue;
+    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
       const int s = n & 1, phase = (n >> 1) & 1;
       ++n;
       if (!mbar_wait_bounded(bar(kWFull + s), phase) || !mbar_wait_bounded(bar(kWSEmpty + s), phase ^ 1)) break;
@@ -762,7 +815,7 @@ cudaError_t launch_weights(const AttnArgs& a, int64_t longest, cudaStream_t s) {
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = allow_shared<kv4_weights_kernel<D>>(Wgt<D>::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kv4_weights_kernel<D>, grid, Wgt<D>::kThreads, Wgt<D>::kSmem, s, a, (int)tiles);
+  return launch_kernel(kv4_weights_kernel<D>, grid, Wgt<D>::kThreads, Wgt<D>::kSmem, s, a);
 }
 
 struct PrefillShape {
