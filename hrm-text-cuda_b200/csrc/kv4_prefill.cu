@@ -659,6 +659,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
   __shared__ uint32_t s_tmem;
   __shared__ __align__(16) float s_lse[4][128];  // negated
   __shared__ int s_lim[4][128];
+  __shared__ int s_whole[4], s_more[4];  // all of the tile's queries see all of the rows; another tile follows
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t base = smem_addr(smem), bar0 = smem_addr(bars);
   auto bar = [&](int i) -> uint32_t { return bar0 + 8 * i; };
@@ -719,13 +720,14 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     uint64_t sum[2] = {0, 0};
     float extra = 0.0f;  // of tiles with masked probabilities
     const uint64_t scale2 = pack_f32x2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
-    int n = 0;
-    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
+    int n = 0, more = 1;  // (`first` < limit: there is a tile)
+    while (more) {
       const int s = n & 1, phase = (n >> 1) & 1, entry = n & 3;
       ++n;
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(kWSFull + s), phase))) break;
       tcgen05_after_sync();
-      const bool whole = first + 128 <= q.lowest;
+      const bool whole = s_whole[entry] != 0;
+      more = s_more[entry];
       uint32_t x[2][32];  // 32 columns are loaded while the 32 before them are worked on
       tmem_load32(x[0], tmem + lanes + 128 * s);
 #pragma unroll
@@ -768,8 +770,10 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
                            in ? src + at + x : src, in);
       }
     };
+    QueryTiles q(see, a.seq, rows, first);
     int n = 0;
-    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
+    bool more = q.find();
+    while (more) {
       const int s = n & 1, phase = (n >> 1) & 1;
       if (!mbar_wait_bounded(bar(kWEmpty + s), phase ^ 1)) break;
       fetch(q.row, s);
@@ -779,6 +783,13 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
       const unsigned row = q.row + t, sq = q.s + t;
       s_lse[n & 3][t] = row < rows ? -a.lse[q_row0 + row] : 0.0f;
       s_lim[n & 3][t] = row < rows ? see.rows((int)(sq < q.seq ? sq : sq % q.seq)) : -1;
+      const bool whole = first + 128 <= q.lowest;
+      q.step(1);
+      more = q.find();
+      if (t == 0) {
+        s_whole[n & 3] = whole;
+        s_more[n & 3] = more;
+      }
       ++n;
       cp_async_wait_all();
       fence_proxy_async_smem();
@@ -787,11 +798,11 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
   } else if (elect_one()) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t kShape = mma_shape(128, 128);
-    int n = 0;
-    for (QueryTiles q(see, a.seq, rows, first); q.find(); q.step(1)) {
+    int n = 0, more = 1;
+    while (more) {
       const int s = n & 1, phase = (n >> 1) & 1;
-      ++n;
       if (!mbar_wait_bounded(bar(kWFull + s), phase) || !mbar_wait_bounded(bar(kWSEmpty + s), phase ^ 1)) break;
+      more = s_more[n++ & 3];
       tcgen05_after_sync();
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
