@@ -214,6 +214,147 @@ void HrmLayerOps::split_gqkv_rope(const CudaSlice<bf16>& gqkv, CudaSlice<bf16>& 
         "split_gqkv_rope");
 }
 
+// ---- the 4-bit KV cache
+namespace {
+
+template <class T>
+CudaSlice<T> alloc_zero(size_t len, cudaStream_t stream) {
+  void* p = nullptr;
+  cuda_check(cudaMalloc(&p, len * sizeof(T) + (len == 0)), "cudaMalloc");
+  CudaSlice<T> s(static_cast<T*>(p), len);
+  cuda_check(cudaMemsetAsync(p, 0, len * sizeof(T), stream), "cudaMemsetAsync");
+  return s;
+}
+
+// The C struct of a cache whose slices have been checked against its sizes.
+hrm_kv4_cache kv4_struct(const HrmLayerOps::Kv4Cache& c, const char* op) {
+  const size_t rows = c.batch * c.kv_heads * c.cache_len;
+  need(c.k_codes, rows * (c.head_dim / 2), op, "k_codes");
+  need(c.v_codes, rows * (c.head_dim / 2), op, "v_codes");
+  need(c.k_scales, rows * (c.head_dim / 32), op, "k_scales");
+  need(c.v_scales, rows * (c.head_dim / 32), op, "v_scales");
+  if (c.weights.device_ptr()) need(c.weights, rows, op, "weights");
+  if (c.positions.device_ptr()) need(c.positions, rows, op, "positions");
+  return hrm_kv4_cache{c.k_codes.device_ptr(),   c.k_scales.device_ptr(), c.v_codes.device_ptr(),
+                       c.v_scales.device_ptr(),  c.weights.device_ptr(),  c.positions.device_ptr(),
+                       (int64_t)c.batch,         (int64_t)c.kv_heads,     (int64_t)c.cache_len,
+                       (int64_t)c.head_dim};
+}
+
+const int32_t* per_sequence(HrmLayerOps::PerSequence p, size_t batch, const char* op, const char* name) {
+  if (p == nullptr) return nullptr;
+  need(*p, batch, op, name);
+  return p->device_ptr();
+}
+
+}  // namespace
+
+CudaSlice<int32_t> HrmLayerOps::htod_copy_i32(const std::vector<int32_t>& host) const {
+  CudaSlice<int32_t> s = alloc_zero<int32_t>(host.size(), stream_);
+  cuda_check(cudaMemcpyAsync(s.device_ptr(), host.data(), host.size() * sizeof(int32_t), cudaMemcpyHostToDevice,
+                             stream_),
+             "cudaMemcpyAsync");
+  cuda_check(cudaStreamSynchronize(stream_), "cudaStreamSynchronize");  // host vector may die after return
+  return s;
+}
+
+HrmLayerOps::Kv4Cache HrmLayerOps::alloc_kv4_cache(size_t batch, size_t kv_heads, size_t cache_len, size_t head_dim,
+                                                   bool track) const {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 192 && head_dim != 256)
+    fail(HrmError::Kind::InvalidInput, HRM_ERR_INVALID_SHAPE,
+         "alloc_kv4_cache: head_dim " + std::to_string(head_dim) + " is not 64, 128, 192 or 256");
+  const size_t rows = batch * kv_heads * cache_len;
+  Kv4Cache c;
+  c.batch = batch;
+  c.kv_heads = kv_heads;
+  c.cache_len = cache_len;
+  c.head_dim = head_dim;
+  c.k_codes = alloc_zero<uint8_t>(rows * (head_dim / 2), stream_);
+  c.v_codes = alloc_zero<uint8_t>(rows * (head_dim / 2), stream_);
+  c.k_scales = alloc_zero<uint32_t>(rows * (head_dim / 32), stream_);
+  c.v_scales = alloc_zero<uint32_t>(rows * (head_dim / 32), stream_);
+  if (track) {
+    c.weights = alloc_zero<float>(rows, stream_);
+    c.positions = alloc_zero<int32_t>(rows, stream_);
+  }
+  return c;
+}
+
+void HrmLayerOps::kv4_update(Kv4Cache& cache, const CudaSlice<bf16>& k, const CudaSlice<bf16>& v, size_t seq_len,
+                             size_t position_offset, size_t cache_offset, PerSequence position_offsets,
+                             PerSequence cache_offsets) const {
+  const hrm_kv4_cache c = kv4_struct(cache, "kv4_update");
+  const size_t n = cache.batch * cache.kv_heads * seq_len * cache.head_dim;
+  need(k, n, "kv4_update", "k");
+  need(v, n, "kv4_update", "v");
+  check(hrm_kv4_update(&c, k.device_ptr(), v.device_ptr(), (int64_t)seq_len, (int64_t)position_offset,
+                       per_sequence(position_offsets, cache.batch, "kv4_update", "position_offsets"),
+                       (int64_t)cache_offset, per_sequence(cache_offsets, cache.batch, "kv4_update", "cache_offsets"),
+                       stream_),
+        "kv4_update");
+}
+
+void HrmLayerOps::split_gqkv_rope_kv4(const CudaSlice<bf16>& gqkv, CudaSlice<bf16>& gate, CudaSlice<bf16>& q,
+                                      CudaSlice<bf16>* k, CudaSlice<bf16>* v, Kv4Cache& cache, size_t seq_len,
+                                      size_t position_offset, size_t cache_offset, PerSequence position_offsets,
+                                      PerSequence cache_offsets) const {
+  const char* op = "split_gqkv_rope_kv4";
+  const hrm_kv4_cache c = kv4_struct(cache, op);
+  const size_t n = cache.batch * seq_len * cache.kv_heads * cache.head_dim;
+  need(gqkv, 4 * n, op, "gqkv");
+  need(gate, n, op, "gate");
+  need(q, n, op, "q");
+  if ((k == nullptr) != (v == nullptr))
+    fail(HrmError::Kind::InvalidInput, HRM_ERR_NULL_POINTER, "split_gqkv_rope_kv4: pass both k and v or neither");
+  if (k) {
+    need(*k, n, op, "k");
+    need(*v, n, op, "v");
+  }
+  const bool use_table = rope_table_.device_ptr() != nullptr && cache.head_dim == config.head_dim &&
+                         (position_offsets != nullptr || position_offset + seq_len <= rope_positions_);
+  check(hrm_split_gqkv_rope_kv4(gqkv.device_ptr(), gate.device_ptr(), q.device_ptr(), k ? k->device_ptr() : nullptr,
+                                v ? v->device_ptr() : nullptr, &c, (int64_t)seq_len, (int64_t)position_offset,
+                                per_sequence(position_offsets, cache.batch, op, "position_offsets"), config.rope_theta,
+                                use_table ? rope_table_.device_ptr() : nullptr,
+                                use_table ? (int64_t)rope_positions_ : 0, (int64_t)cache_offset,
+                                per_sequence(cache_offsets, cache.batch, op, "cache_offsets"), stream_),
+        op);
+}
+
+void HrmLayerOps::kv4_attention(const CudaSlice<bf16>& q, Kv4Cache& cache, const CudaSlice<bf16>* gate,
+                                CudaSlice<bf16>& out, size_t num_heads, size_t seq_len, size_t cache_offset,
+                                size_t prefix_len, float softmax_scale, bool accumulate,
+                                PerSequence cache_offsets) const {
+  const char* op = "kv4_attention";
+  const hrm_kv4_cache c = kv4_struct(cache, op);
+  const size_t n = cache.batch * num_heads * seq_len * cache.head_dim;
+  need(q, n, op, "q");
+  need(out, n, op, "out");
+  if (gate) need(*gate, n, op, "gate");
+  int64_t bytes = 0;
+  check(hrm_kv4_attention_workspace(&c, (int64_t)num_heads, (int64_t)seq_len, accumulate, &bytes), op);
+  if (workspace_.len() < (size_t)bytes) {  // freeing the old one waits for the calls that use it
+    workspace_ = CudaSlice<uint8_t>();
+    workspace_ = alloc_zero<uint8_t>((size_t)bytes, stream_);
+  }
+  check(hrm_kv4_attention(q.device_ptr(), &c, gate ? gate->device_ptr() : nullptr, out.device_ptr(),
+                          (int64_t)num_heads, (int64_t)seq_len, (int64_t)cache_offset,
+                          per_sequence(cache_offsets, cache.batch, op, "cache_offsets"), (int64_t)prefix_len,
+                          softmax_scale, accumulate, workspace_.device_ptr(), (int64_t)workspace_.len(), stream_),
+        op);
+}
+
+void HrmLayerOps::kv4_evict(Kv4Cache& cache, size_t length, size_t budget, int64_t protect_from,
+                            CudaSlice<int32_t>& new_lengths, PerSequence lengths, PerSequence protect_froms) const {
+  const char* op = "kv4_evict";
+  const hrm_kv4_cache c = kv4_struct(cache, op);
+  need(new_lengths, cache.batch, op, "new_lengths");
+  check(hrm_kv4_evict(&c, &c, (int64_t)length, per_sequence(lengths, cache.batch, op, "lengths"), (int64_t)budget,
+                      protect_from, per_sequence(protect_froms, cache.batch, op, "protect_froms"),
+                      new_lengths.device_ptr(), stream_),
+        op);
+}
+
 void HrmLayerOps::build_rope_table(size_t max_positions) {
   void* p = nullptr;
   const size_t n = max_positions * config.head_dim;

@@ -180,6 +180,44 @@ class HrmLayerOps {
                        CudaSlice<bf16>& v, CudaSlice<bf16>* k_cache, CudaSlice<bf16>* v_cache, size_t batch_size,
                        size_t seq_len, size_t num_heads, size_t head_dim, size_t position_offset, size_t cache_len,
                        size_t cache_offset) const;
+  // ---- the 4-bit KV cache (include/hrm_ops.h has the format and the formulas; the
+  // reference's cache is bf16)
+  struct Kv4Cache {
+    size_t batch = 0, kv_heads = 0, cache_len = 0, head_dim = 0;
+    CudaSlice<uint8_t> k_codes, v_codes;     // [batch, kv_heads, cache_len, head_dim / 2]
+    CudaSlice<uint32_t> k_scales, v_scales;  // [batch, kv_heads, cache_len, head_dim / 32] pairs of bf16
+    CudaSlice<float> weights;                // [batch, kv_heads, cache_len] where asked for, else empty
+    CudaSlice<int32_t> positions;            // likewise
+  };
+  // Per-sequence offsets or lengths in device memory (one int32 each) take the place
+  // of the host value beside them; null: the host value holds for all.
+  using PerSequence = const CudaSlice<int32_t>*;
+  CudaSlice<int32_t> htod_copy_i32(const std::vector<int32_t>& host) const;
+  // A cache of zeros; track: with weights and positions, as kv4_attention's accumulate
+  // and kv4_evict need them.
+  Kv4Cache alloc_kv4_cache(size_t batch, size_t kv_heads, size_t cache_len, size_t head_dim, bool track = false) const;
+  // kv_cache_update (src/lib.rs:706-747) into a 4-bit cache.
+  void kv4_update(Kv4Cache& cache, const CudaSlice<bf16>& k, const CudaSlice<bf16>& v, size_t seq_len,
+                  size_t position_offset, size_t cache_offset, PerSequence position_offsets = nullptr,
+                  PerSequence cache_offsets = nullptr) const;
+  // split_gqkv_rope into a 4-bit cache of as many heads; k and v, both or neither
+  // null, receive the values that the cache now stands for.
+  void split_gqkv_rope_kv4(const CudaSlice<bf16>& gqkv, CudaSlice<bf16>& gate, CudaSlice<bf16>& q, CudaSlice<bf16>* k,
+                           CudaSlice<bf16>* v, Kv4Cache& cache, size_t seq_len, size_t position_offset,
+                           size_t cache_offset, PerSequence position_offsets = nullptr,
+                           PerSequence cache_offsets = nullptr) const;
+  // mha, mha_decode and (with gate) apply_attn_gate over a 4-bit cache: out is [batch,
+  // seq_len, num_heads, head_dim].  The layer keeps the workspace between calls; a
+  // call that needs more of it than any before allocates it, so make one of the
+  // largest before capturing a graph.
+  void kv4_attention(const CudaSlice<bf16>& q, Kv4Cache& cache, const CudaSlice<bf16>* gate, CudaSlice<bf16>& out,
+                     size_t num_heads, size_t seq_len, size_t cache_offset, size_t prefix_len, float softmax_scale,
+                     bool accumulate = false, PerSequence cache_offsets = nullptr) const;
+  // Keeps the budget rows of the largest weight (and those at positions >=
+  // protect_from) of each head's first `length`, in place; new_lengths: [batch].
+  void kv4_evict(Kv4Cache& cache, size_t length, size_t budget, int64_t protect_from, CudaSlice<int32_t>& new_lengths,
+                 PerSequence lengths = nullptr, PerSequence protect_froms = nullptr) const;
+
   // ---- the layer loop's residual / norm schedule
   // Scratch of one module pass over `rows` tokens (the reference's
   // ScratchBuffers, src/lib.rs:86-112): the residual stream x, the normed
@@ -241,6 +279,7 @@ class HrmLayerOps {
   cudaStream_t stream_ = nullptr;
   CudaSlice<float> rope_table_;
   size_t rope_positions_ = 0;
+  mutable CudaSlice<uint8_t> workspace_;  // kv4_attention's; its calls are queued on one stream
 };
 
 }  // namespace hrm
