@@ -33,8 +33,6 @@ Offset = Union[int, torch.Tensor]
 # decode step makes one such call per layer and operator).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -202,9 +200,9 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
     cache_offset counts the rows before the queries' own tokens, which the cache
     already holds: query i sees rows j <= cache_offset + i, and those below
     prefix_len.  gate [b, s, heads, d] multiplies by its sigmoid; scale defaults
-    to 1 / sqrt(head_dim); accumulate adds the probabilities to cache.weights
-    (`workspace`: a uint8 tensor of at least kv4_attention_workspace bytes, else
-    one is allocated on the current stream).  A sequence with a negative
+    to 1 / sqrt(head_dim); accumulate adds the probabilities to cache.weights.
+    workspace: a uint8 tensor of at least kv4_attention_workspace bytes, else one is
+    allocated for the call, on the launch's stream.  A sequence with a negative
     cache_offset whose queries see nothing gives 0.  src/lib.rs:632-704.
     """
     _need(q, "q")
