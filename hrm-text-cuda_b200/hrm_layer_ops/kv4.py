@@ -165,9 +165,8 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
     s = gqkv.shape[1]
     if out is None:
-        new, kv = gqkv.new_empty, (b, h, s, d)
-        gate, q = new((b, s, h, d)), new(kv)
-        k, v = (new(kv), new(kv)) if keep_kv else (None, None)
+        gate, q = gqkv.new_empty((b, s, h, d)), gqkv.new_empty((b, h, s, d))
+        k, v = (torch.empty_like(q), torch.empty_like(q)) if keep_kv else (None, None)
         given = ()
     else:
         gate, q, k, v = given = tuple(out)
@@ -210,16 +209,16 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[1] % hk or q.shape[1] == 0:
         raise ValueError(f"q must be [{b}, a multiple of {hk} heads, seq, {d}]")
     h, s = q.shape[1], q.shape[2]
+    if gate is not None:
+        _need(gate, "gate")
+        if gate.numel() != q.numel():
+            raise ValueError("gate has the wrong size")
     if out is None:
         out = q.new_empty((b, s, h, d))
     else:
         _need(out, "out")
         if out.numel() != q.numel():
             raise ValueError("out has the wrong size")
-    if gate is not None:
-        _need(gate, "gate")
-        if gate.numel() != q.numel():
-            raise ValueError("gate has the wrong size")
     off, off_t = _offset(cache_offset, "cache_offset", b)
     if accumulate and cache.weights is None:
         raise ValueError("accumulate needs a cache with weights (kv4_cache(..., track=True))")
@@ -270,10 +269,11 @@ def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offse
     length, length_t = _offset(lengths, "lengths", b)
     protect, protect_t = _offset(protect_from, "protect_from", b)
     if new_lengths is None:
-        new_lengths = torch.empty(b, dtype=torch.int32, device=cache.device)
-    _need(new_lengths, "new_lengths", (torch.int32,))
-    if new_lengths.numel() != b:
-        raise ValueError("new_lengths must have one value per sequence")
+        new_lengths = cache.positions.new_empty(b)
+    else:
+        _need(new_lengths, "new_lengths", (torch.int32,))
+        if new_lengths.numel() != b:
+            raise ValueError("new_lengths must have one value per sequence")
     _launch("hrm_kv4_evict", cache.device, (to.k_codes, length_t, protect_t, new_lengths), stream, cache._ref, to._ref,
             length, _ptr(length_t), budget, protect, _ptr(protect_t), _ptr(new_lengths))
     return new_lengths
