@@ -986,10 +986,13 @@ int64_t shares_for(int64_t head_dim) {
 template <int D, bool ONE>
 cudaError_t launch_decode(const AttnArgs& a, int64_t longest, float* parts, cudaStream_t s) {
   if (longest <= kSplitRows) {
-    // CTAs per item: while all of them fit at once and each warp has a tile
+    // CTAs per item: while each has an SM for itself and its warps a tile each.  Two on
+    // an SM pay from some 2000 rows on (128 items of 6 query rows, D = 64, one CTA against
+    // two of them each: 600 rows 8.4 against 10.2 us, 1250 10.8 against 11.8, ragged
+    // up to 2500 15.1 against 14.2).
     constexpr int kWarps = kClusterWarps;
     using T = Cta<D, kWarps>;
-    const int64_t items = items_of(a), slots = (int64_t)device_sm_count() * T::kPerSm;
+    const int64_t items = items_of(a), slots = (int64_t)device_sm_count() * (longest > 2048 ? T::kPerSm : 1);
     int count = 1;
     while (count < kClusterMax && items * (count + 1) <= slots && (int64_t)kTileRows * kWarps * count < longest) ++count;
     const cudaError_t e = allow_shared<kv4_decode_kernel<D, ONE>>(T::kSmem);
