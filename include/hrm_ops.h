@@ -354,9 +354,10 @@ int hrm_kv4_attention_workspace(const hrm_kv4_cache* cache, int64_t num_heads, i
  * new_lengths[b] = min(n, budget); it must not overlap lengths.
  * `out` may be the cache itself (in place: only the moved rows are written) or
  * another cache of at least min(budget, n) rows, with no buffer shared.  Both need
- * weights and positions.  Limit: 4 * min(budget, n - budget) + n / 8 bytes
- * (n the host length, or cache_len with `lengths`) may not pass 170 KB
- * (HRM_ERR_SCRATCH_LIMIT).  No reference counterpart.                          */
+ * weights and positions.  Limit: 4 * min(budget, n - budget) + 3 n / 8 bytes
+ * (n the host length, or cache_len with `lengths`) may not pass 156 KiB
+ * (HRM_ERR_SCRATCH_LIMIT): 67000 rows at any budget, 400000 rows for a budget of
+ * 2000.  No reference counterpart.                                             */
 int hrm_kv4_evict(const hrm_kv4_cache* cache, const hrm_kv4_cache* out, int64_t length, const int32_t* lengths,
                   int64_t budget, int64_t protect_from, const int32_t* protect_froms, int32_t* new_lengths,
                   hrm_stream_t stream);

@@ -53,6 +53,45 @@ def test_prompts_against_the_plain_form(cuda, b, hk, group, s, n, d, prefix, rag
     assert ops.wait_timeouts() == 0
 
 
+def test_prompt_and_eviction_past_four_gigabytes(cuda):
+    """Offsets past 2^32 bytes in the prompt's kernels and in the eviction: the last head
+    of a large cache."""
+    b, h, n, d, s = 3, 12, 1 << 20, 256, 70
+    c = ops.kv4_cache(b, h, n, d, track=True)
+    assert c.k_codes.numel() > 1 << 32
+    small = filled(1, 1, 4096, d, 95)
+    for name, t in buffers(c).items():
+        t[-1, -1, -4096:] = buffers(small)[name][0, 0]
+        t[-1, -1, :4096] = buffers(small)[name][0, 0]
+    c.weights[-1, -1, 4096:].zero_()
+    q = rand((b, h, s, d), 97)
+    off = torch.tensor([-s, -s, n - s], dtype=torch.int32, device="cuda")
+    w0 = c.weights[-1, -1].double()
+    got = ops.kv4_attention(q, c, off, accumulate=True)
+    assert not bool(got[:2].any()) and ops.wait_timeouts() == 0
+    kk, vv = ref.values(c.k_codes[-1, -1], c.k_scales[-1, -1]), ref.values(c.v_codes[-1, -1], c.v_scales[-1, -1])
+    x = q[-1, -1].double() @ kk.T / 16
+    seen = torch.arange(n, device="cuda")[None] <= torch.arange(n - s, n, device="cuda")[:, None]
+    p = torch.softmax(x.masked_fill(~seen, -float("inf")), 1)
+    want, spread = p @ vv, p @ vv.abs()
+    # fp32 sums of 2^20 rows, 16 to an addition, at most 2^-23 each: 2^-7; of 128 to an addition in l: 2^-10
+    assert bool(((got[-1, :, -1].double() - want).abs() <= U * want.abs() + spread * (2.0**-6 + U)).all())
+    err, w = (c.weights[-1, -1].double() - w0 - p.sum(0)).abs(), p.sum(0)
+    assert bool((err <= 2.0**-9 * w + 100 * 2.0**-23 * (w0 + w)).all())
+    del kk, vv, x, seen, p
+    # the first 4096 rows of each head, of which the last head's have weights
+    want = ref.evict(c.weights[-1, -1, :4096].cpu().numpy(), c.positions[-1, -1, :4096].cpu().numpy(), 4096, 1000, 4090)
+    before = {name: t[-1, -1, :4096].clone() for name, t in buffers(c).items()}
+    lengths = ops.kv4_evict(c, 4096, 1000, 4090)
+    assert lengths.tolist() == [1000] * b
+    for name, t in buffers(c).items():
+        same(t[-1, -1, :1000], before[name][want], name)
+    del c, before
+    torch.cuda.empty_cache()
+    with pytest.raises(ops.HrmError):  # more rows than an eviction takes
+        ops.kv4_evict(ops.kv4_cache(1, 1, 500000, 64, track=True), 500000, 100, 0)
+
+
 @pytest.mark.parametrize("s", [1, 40])
 def test_gate_extremes(cuda, s):
     """sigmoid(gate) at its ends; what it makes smaller than 2^-126 may be 0."""
