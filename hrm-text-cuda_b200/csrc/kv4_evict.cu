@@ -16,6 +16,9 @@
 // and ends early when a digit's border leaves exactly `budget` rows.  Rows whose key
 // is the threshold are then taken in row order.  When a single row must go (a
 // decode step) it is one CTA-wide minimum instead.
+//
+// Measured: 64 x 16 heads, one of 1025 rows each, 10 us with the write of the new row; 12 heads, 32768 rows to 4096 of D = 128,
+// 28 us; 16 x 16 heads, up to 5000 rows to 1111 of D = 64, 29 us.
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -78,7 +81,9 @@ __device__ __forceinline__ int cta_scan(int x, int* buf, int* total) {
 // Rows that can move at most, and the dynamic shared memory: counts of the three
 // digits, the cluster's sums of one, per 32 rows of the CTA a mask and two ranks,
 // and the freed places in order (in the cluster's first CTA).
-inline int64_t evict_moves(int64_t n, int64_t budget) { return n <= budget ? 0 : (n - budget < budget ? n - budget : budget); }
+inline int64_t evict_moves(int64_t n, int64_t budget) {
+  return n <= budget ? 0 : (n - budget < budget ? n - budget : budget);
+}
 constexpr size_t kSharedMost = 200 * 1024;
 inline size_t evict_shared(int64_t groups, int64_t moves) { return 4 * (size_t)(4 * kBins + 3 * groups + moves); }
 
@@ -87,7 +92,8 @@ inline size_t evict_shared(int64_t groups, int64_t moves) { return 4 * (size_t)(
 // rows [c, c + 1) * W * steps * 32; groups of 32 rows go to the warps in turn, so that the
 // copies are even over the warps wherever the rows that stay lie.
 template <int W, int K>
-__global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2) kv4_evict_kernel(const EvictArgs a, const int count, const int steps_at_most) {
+__global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
+    kv4_evict_kernel(const EvictArgs a, const int count, const int steps_at_most) {
   extern __shared__ __align__(16) int shared[];
   int* hist = shared;                                                 // [3][kBins]
   int* sums = shared + 3 * kBins;                                     // [kBins]: the cluster's
@@ -335,7 +341,9 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2) kv4_evict_kernel(const
     const uint32_t low = places(g), mask = masks[g], moving = mask & ~low, todo = a.in_place ? moving : mask;
     if (todo >> lane & 1u) {
       const int at = move_at[g] + __popc(moving & ((1u << lane) - 1));
-      const int to = low >> lane & 1u ? first + lane : (count == 1 ? freed[at] : *cluster.map_shared_rank(freed + at, 0));
+      const int to = low >> lane & 1u
+                         ? first + lane
+                         : (count == 1 ? freed[at] : *cluster.map_shared_rank(freed + at, 0));
       s_copy[warp][listed + __popc(todo & ((1u << lane) - 1))] = make_int2(first + lane, to);
     }
     listed += __popc(todo);
@@ -409,7 +417,9 @@ cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_pla
   a.code_pieces = (int)(head_dim / 32);
   a.in_place = in_place;
   const int64_t n = lengths ? from.cache_len : (length < from.cache_len ? length : from.cache_len);
-  // CTAs per head: while they leave room on the GPU (2 of 512 threads per SM) and have 2048 rows each
+  // CTAs per head: while they leave room on the GPU (2 of 512 threads per SM) and have 2048 rows
+  // each (12 heads: 2048 rows on one CTA 11.4 us, on two 15.8; 4096 17.3 and 18.0; 8192 25.6
+  // and, on four, 18.0; 32768 198 and, on eight, 27.7)
   int count = 1;
   while (count < 8 && batch * kv_heads * count * 2 <= 2 * device_sm_count() && n >= 2048 * count * 2) count *= 2;
   const int64_t mine = (n + count - 1) / count;

@@ -45,9 +45,14 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 // Query rows of one kv head up to which the probabilities are added to the
-// weights by the decode kernel itself (one block of rows holds them all).
+// weights by the decode kernel itself (one block of rows holds them all).  It keeps the
+// scores for that; the kernel that computes them again takes longer (16 x 16 heads
+// over 8192 rows, 1 query row: 87 us against 433; 8 rows: 156 against 452).
 constexpr int64_t kDecodeRows = 8;
-// Query rows of one kv head up to which the decode kernel serves them, in blocks of 8.
+// Query rows of one kv head up to which the decode kernel serves them, in blocks of 8 (12
+// heads of 128, decode kernel against the prompts': 9 rows over 1024 9.8 and 16.9 us, 32
+// rows over 1024 13.6 and 16.6, over 8192 33.9 and 26.0; a batch of 8, 32 rows over
+// 8192 131 and 154).
 constexpr int64_t kChunkRows = 32;
 
 // What every attention kernel is given.

@@ -4,7 +4,7 @@
 //
 // A CTA owns NQ x 128 query rows of one kv head and walks its share of the cache in
 // tiles of N rows: NQ = 2 and N = 128 up to head_dim 128, 1 and 64 above, where the
-// operands of two stages fill the shared memory.  Two kinds of warps work at once, handing tiles over by
+// operands of two stages fill the shared memory.  Three kinds of warps work at once, handing tiles over by
 // mbarriers:
 //   * 4 warps dequantise: codes and scales from global memory (the next tile's are
 //     loaded while this one is converted), bf16 operands to shared memory, two
@@ -12,17 +12,20 @@
 //     two cache rows' half words put together before the conversion, so that both
 //     operands are K-major.
 //   * 4 warps per query tile do the softmax, a thread per row, the row in registers:
-//     no shuffles.  One of their threads issues the tile's products: S = Q K^T (128 x N,
-//     accumulated in tensor memory) and O += P V with P read from tensor memory, where
-//     it replaces S.  With NQ = 2 the products of one query tile run while the other's
-//     softmax does.  (A warp of its own for the products would make 13 warps, and 4 on
-//     one scheduler leave a thread 128 registers: too few for a row of 128.)  O is
+//     no shuffles.  P goes to tensor memory, over S, in two halves.  O is
 //     rescaled only when a row's maximum has grown by more than 8 (in log2 units)
 //     since its last rescale: until then probabilities may be as large as 2^8,
 //     which neither the bf16 P nor the fp32 sums mind.
-// What bounds it: a tile costs 128 exponentials per row on a unit of 16 per clock,
-// as long as its two products on the tensor cores; the conversion, 1.6 instructions
-// per element, is a quarter of that for 256 query rows.
+//   * one thread issues the products, S = Q K^T (128 x N, accumulated in tensor memory)
+//     and O += P V with P read from tensor memory: with NQ = 2 those of one query tile
+//     run while the other's softmax does.
+// What bounds it: a tile costs 128 exponentials per row on a unit of 16 per clock
+// (2048 cycles for 256 rows), as long as its products on the tensor cores; but a query
+// tile's softmax waits for its own products, P being where S was, so that a tile takes
+// 3400 cycles of softmax and products in turn, the other query tile's in between.
+// Measured (D = 128): 512 queries of 16 heads over 8192 rows 50 us (710 TFLOP/s); 2 x
+// 4096 queries of 12 heads with gate, causal past a prefix of 1000, 125 us (870), and
+// the weights' kernel below 96.
 // P is rounded to bf16 (2^-8 of itself, the sum l is of the unrounded ones): the
 // operand's type; the error it adds to an output is that of the output's own
 // rounding at most.
@@ -77,7 +80,8 @@ __device__ __forceinline__ uint4 paired_order(const uint4& v) {
 
 // Query rows [r0, + count) of a kv head: the highest and the lowest number of cache
 // rows that one of them sees (rows past the last: none).
-__device__ __forceinline__ int2 row_limits(const Visible& see, unsigned seq, unsigned rows, unsigned r0, unsigned count) {
+__device__ __forceinline__ int2 row_limits(const Visible& see, unsigned seq, unsigned rows, unsigned r0,
+                                           unsigned count) {
   const unsigned r1 = min(r0 + count, rows) - 1;
   const unsigned g0 = r0 / seq, s0 = r0 - g0 * seq, g1 = r1 / seq, s1 = r1 - g1 * seq;
   return make_int2(see.rows((int)(g0 == g1 ? s1 : seq - 1)),
@@ -161,7 +165,8 @@ struct Codes {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int sel = h == 0 ? 0x5410 : 0x7632;
-        const uint32_t xa = __byte_perm(vget(v[0], w), vget(v[1], w), sel), xb = __byte_perm(vget(v[2], w), vget(v[3], w), sel);
+        const uint32_t xa = __byte_perm(vget(v[0], w), vget(v[1], w), sel);
+        const uint32_t xb = __byte_perm(vget(v[2], w), vget(v[3], w), sel);
         const int d = 32 * p + 8 * w + 4 * h;
         auto put = [&](int e, uint32_t ya, uint32_t yb) {
           *reinterpret_cast<uint2*>(panel + panel_piece(d + e, (q & 15) / 2)) =
@@ -609,8 +614,11 @@ __global__ void __launch_bounds__(kM) kv4_prefill_join_kernel(const AttnArgs a, 
 // over its columns by itself -- no atomics, no shuffles, the same sum from call to
 // call.  A CTA owns 128 cache rows, dequantised once; 4 warps copy the query tiles
 // to shared memory (cp.async, two stages), one thread issues the products into two
-// buffers of tensor memory, 4 warps take the exponentials, 128 per row and tile,
-// which bound it.  Up to head_dim 128 two CTAs share an SM.
+// buffers of tensor memory, 4 warps take the exponentials, 128 per row and tile.  Up
+// to head_dim 128 two CTAs share an SM: a pair of tiles takes them 2600 cycles, 2048 of
+// exponentials.  2 x 4096 queries of 12 heads of 128: 96 us (one CTA of 256 cache rows
+// instead of two of 128, with half the copies: 116; every third or fourth pair of exponentials
+// by a polynomial: 94 to 95).
 template <int D>
 struct Wgt {
   static constexpr int kK = 0, kBytes = 128 * D * 2, kQ = kBytes;  // keys; two stages of queries
@@ -738,10 +746,13 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint4 lse = *reinterpret_cast<const uint4*>(&s_lse[entry][32 * c + 4 * i]);
-            const uint64_t y0 = fma_f32x2(pack_f32x2(x[c & 1][4 * i], x[c & 1][4 * i + 1]), scale2, pack_f32x2(lse.x, lse.y));
-            const uint64_t y1 = fma_f32x2(pack_f32x2(x[c & 1][4 * i + 2], x[c & 1][4 * i + 3]), scale2, pack_f32x2(lse.z, lse.w));
-            sum[0] = add_f32x2(sum[0], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y0))), __float_as_uint(exp2_approx(hi_f32(y0)))));
-            sum[1] = add_f32x2(sum[1], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y1))), __float_as_uint(exp2_approx(hi_f32(y1)))));
+            const uint32_t* u = &x[c & 1][4 * i];
+            const uint64_t y0 = fma_f32x2(pack_f32x2(u[0], u[1]), scale2, pack_f32x2(lse.x, lse.y));
+            const uint64_t y1 = fma_f32x2(pack_f32x2(u[2], u[3]), scale2, pack_f32x2(lse.z, lse.w));
+            sum[0] = add_f32x2(sum[0], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y0))),
+                                                  __float_as_uint(exp2_approx(hi_f32(y0)))));
+            sum[1] = add_f32x2(sum[1], pack_f32x2(__float_as_uint(exp2_approx(lo_f32(y1))),
+                                                  __float_as_uint(exp2_approx(hi_f32(y1)))));
           }
         } else {
 #pragma unroll
@@ -844,9 +855,16 @@ PrefillShape prefill_shape(int64_t batch_kv_heads, int64_t rows, int64_t head_di
 template <int D, int NQ>
 cudaError_t launch_prefill(const AttnArgs& a, const PrefillShape& p, int64_t longest, float* parts, cudaStream_t s) {
   using T = Pre<D, NQ>;
-  // One CTA per SM: items that leave SMs idle are split, to 4 tiles at least.
+  // One CTA per SM: items that leave SMs idle are split, to 2 tiles at least (12 heads, 64
+  // queries over 2048 rows: 15.0 us, to 4 tiles 17.6, 256 over 1024 15.8 and 19.4; to 1 tile 256
+  // over 2048 24.6 against 18.3), and into more than 8 parts, whose joining waits for
+  // more reads, only past 64 tiles (256 queries over 4096 rows in 8 parts 22.4, in 12
+  // 26.6; over 16384 47.0 and 43.9).
+  const int64_t most = longest <= 64 * T::kN ? 8 : INT32_MAX;
   PrefillSplit split{1, parts};
-  while (p.items * (split.count + 1) <= device_sm_count() && (split.count + 1) * 4 * T::kN <= longest) ++split.count;
+  while (split.count < most && p.items * (split.count + 1) <= device_sm_count() &&
+         (split.count + 1) * 2 * T::kN <= longest)
+    ++split.count;
   if (p.items * split.count > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaError_t e = allow_shared<kv4_prefill_kernel<D, NQ>>(T::kSmem);
   if (e == cudaSuccess && NQ == 2) e = has_registers<kv4_prefill_kernel<D, NQ>>(T::kLaunchRegs);
