@@ -12,6 +12,7 @@ import torch
 import hrm_layer_ops as ops
 import kv4_reference as ref
 from hrm_layer_ops import module
+import test_kv4_gpu as base
 from test_kv4_gpu import U, buffers, filled, rand, run_attention, same, snapshot
 
 pytestmark = pytest.mark.gpu
@@ -51,6 +52,30 @@ def test_prompts_against_the_plain_form(cuda, b, hk, group, s, n, d, prefix, rag
     got = ops.kv4_attention(q, c, off, gate=gate, prefix_len=prefix, accumulate=True)
     check_vectorised(c, q, off, gate, prefix, got, w0)
     assert ops.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("b,hk,group,s,n,d,ragged", [
+    (1, 2, 1, 4, 13000, 128, False), (3, 1, 4, 2, 12800, 256, True), (2, 1, 2, 9, 14000, 64, False),
+    (1, 1, 1, 3, 13000, 192, False), (5, 2, 1, 1, 15000, 128, True), (1, 1, 4, 8, 12289, 128, True),
+    (80, 2, 1, 2, 4200, 64, True)])
+def test_long_caches_in_equal_shares(cuda, b, hk, group, s, n, d, ragged):
+    """Caches past what a cluster serves, with one and several query rows per item."""
+    base.test_attention_long_caches(cuda, b, hk, group, s, n, d, ragged)
+
+
+def test_equal_shares_nan_rows(cuda):
+    """As test_long_caches_nan_rows_and_lse_order, in the equal shares."""
+    n, d, s = 14000, 128, 4
+    c = filled(1, 2, n, d, 33)
+    q = rand((1, 2, s, d), 34)
+    clean = ops.kv4_attention(q, c, n - s)
+    c.v_scales[:, :, n - 1, 1, 0] = float("nan")
+    got = ops.kv4_attention(q, c, n - s)
+    same(got[:, :-1], clean[:, :-1])
+    nan = torch.isnan(got[0, -1])
+    want = torch.zeros_like(nan)
+    want[:, 32:64] = True
+    assert torch.equal(nan, want)
 
 
 def test_prompt_and_eviction_past_four_gigabytes(cuda):
