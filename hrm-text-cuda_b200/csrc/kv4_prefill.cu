@@ -49,21 +49,27 @@ template <int D, int NQ>
 struct Pre {
   static constexpr int kN = tile_rows<D>();  // cache rows of a tile
   static constexpr int kGroups = D / kKv4Group;
-  static constexpr int kSoftmax = NQ * 128, kFill = 128;
-  static constexpr int kThreads = kSoftmax + kFill + (NQ == 2 ? 128 : 32);
-  // NQ = 2: 4 warps on each scheduler would leave a thread 128 registers, too few for
-  // a row of 128 scores.  The warpgroups share the launch's registers out again
-  // (chunk of 512 over 8192: 51 us; 168 + 104 + 72: 60; 152 + 120 + 88: 60).
-  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kFillRegs = 120, kMmaRegs = 72;
-  static_assert(NQ == 1 || 2 * kSoftmaxRegs + kFillRegs + kMmaRegs <= 4 * kLaunchRegs);
+  // Warpgroups: NQ of softmax; one that fills k and v, or (NQ = 1, where a tile has half
+  // the softmax but all the filling) one for each; one for the products' thread.
+  static constexpr int kSoftmax = NQ * 128, kFill = (3 - NQ) * 128;
+  static constexpr int kThreads = kSoftmax + kFill + 128;
+  // 4 warps on each scheduler leave a thread 128 registers, too few for a row of 128
+  // scores.  The warpgroups share the launch's registers out again (NQ = 2, chunk of 512
+  // over 8192: 51 us; 168 + 104 + 72: 60; 152 + 120 + 88: 60).
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = NQ == 2 ? 160 : 184, kFillRegs = 120, kMmaRegs = 72;
+  static_assert(NQ * kSoftmaxRegs + (3 - NQ) * kFillRegs + kMmaRegs <= 4 * kLaunchRegs);
   static constexpr int kQ = 0, kQBytes = kM * D * 2;              // per query tile
   static constexpr int kK = NQ * kQBytes, kKBytes = kN * D * 2;   // per stage
   static constexpr int kV = kK + 2 * kKBytes, kVBytes = D * kN * 2;
   static constexpr int kSmem = kV + 2 * kVBytes + 1024;  // + alignment of the panels
-  static constexpr uint32_t kColumns = tmem_columns(NQ * (kN + D));  // S of each tile, then O of each
+  // A single query tile has two buffers of S, which take turns: S of the next cache tile
+  // is computed during the softmax of this one.
+  static constexpr int kSBufs = 3 - NQ;
+  static constexpr int kOAt = NQ * kSBufs * kN;
+  static constexpr uint32_t kColumns = tmem_columns(kOAt + NQ * D);  // S of each tile, then O of each
 };
 
-// Barriers, in order.
+// Barriers, in order: pairs by stage; S and P by query tile, or by buffer of S; O by query tile.
 enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPHalf = 10, kPFull = 12, kOFull = 14, kBars = 16 };
 
 struct PrefillSplit {
@@ -246,9 +252,9 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
-        mbar_init(bar(kKFull + i), T::kFill);
+        mbar_init(bar(kKFull + i), 128);
         mbar_init(bar(kKEmpty + i), 1);
-        mbar_init(bar(kVFull + i), T::kFill);
+        mbar_init(bar(kVFull + i), 128);
         mbar_init(bar(kVEmpty + i), 1);
         mbar_init(bar(kSFull + i), 1);
         mbar_init(bar(kPHalf + i), kM);
@@ -268,10 +274,10 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
 
   if (warp < kFillFirst) {
     // ---------------------------------------------------------------- softmax
-    if (NQ == 2) take_registers<T::kSoftmaxRegs>();
+    take_registers<T::kSoftmaxRegs>();
     const int qt = warp / 4, r = qt * kM + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + qt * kN, o_at = tmem + lanes + NQ * kN + qt * D;
+    const uint32_t o_at = tmem + lanes + T::kOAt + qt * D;
     const int lim = row0 + r < rows ? see.rows((int)((row0 + r) % a.seq)) : -1;
     const float scale = a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2);
     float m = -INFINITY, l = 0.0f;  // m: of the unscaled scores, as of the last rescale
@@ -279,7 +285,9 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int first = (j0 + j) * kN;
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kSFull + qt), j & 1));
+      const int buf = T::kSBufs == 2 ? j & 1 : qt, turn = T::kSBufs == 2 ? (j >> 1) & 1 : j & 1;
+      const uint32_t s_at = tmem + lanes + buf * kN;
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kSFull + buf), turn));
       if (!ok) break;
       tcgen05_after_sync();
       uint32_t s[kN];
@@ -301,8 +309,9 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
           x[(i >> 1) & 3] = max3_nan(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         top = max3_nan(x[0], x[1], max_nan(x[2], x[3]));
       }
-      // Grown by more than the slack (or from nothing, or NaN): rescale.  S of this
-      // tile is complete, so every product issued before it is, O's among them.
+      // Grown by more than the slack (or from nothing, or NaN): rescale.  With one buffer
+      // of S, S of this tile is complete, so every product issued before it is, O's among
+      // them; with two, O's of the tile before may still run.
       const bool grown = !(top <= m + kSlack / scale);
       if (__any_sync(0xffffffffu, grown)) {
         const float to = grown ? max_nan(top, m) : m;
@@ -310,6 +319,11 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         if (grown) {
           l *= f;
           m = to;
+        }
+        if (T::kSBufs == 2 && j > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kVEmpty + ((j - 1) & 1)), ((j - 1) >> 1) & 1));
+          if (!ok) break;
+          tcgen05_after_sync();
         }
         if (j > 0) {
           const float by = grown ? f : 1.0f;
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         if (c + 1 == kN / 64 || c + 1 == kN / 32) {
           tmem_wait_store();
           tcgen05_before_sync();
-          mbar_arrive(bar((c + 1 == kN / 64 ? kPHalf : kPFull) + qt));
+          mbar_arrive(bar((c + 1 == kN / 64 ? kPHalf : kPFull) + buf));
         }
       }
       const uint64_t both = add_f32x2(sum[0], sum[1]);
@@ -451,8 +465,9 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     }
   } else if (fills) {
     // --------------------------------------------------------------- filling
-    if (NQ == 2) give_registers<T::kFillRegs>();
-    const int t = tid - T::kSoftmax;
+    give_registers<T::kFillRegs>();
+    const int t = tid & 127;
+    const bool fills_k = NQ == 2 || warp < kFillFirst + 4, fills_v = NQ == 2 || !fills_k;
     const int64_t head_row = (int64_t)bh * a.c.cache_len;
     const uint8_t* kc = a.c.k_codes + head_row * (D / 2);
     const uint8_t* vc = a.c.v_codes + head_row * (D / 2);
@@ -460,67 +475,81 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     const uint32_t* vs = a.c.v_scales + head_row * T::kGroups;
     Codes<D, kN> c;
     if (n > 0) {
-      c.fetch_k(kc, ks, j0 * kN, limit, t);
-      c.fetch_v(vc, vs, j0 * kN, limit, t);
+      if (fills_k) c.fetch_k(kc, ks, j0 * kN, limit, t);
+      if (fills_v) c.fetch_v(vc, vs, j0 * kN, limit, t);
     }
     for (int j = 0; j < n; ++j) {
       const int first = (j0 + j) * kN, s = j & 1, phase = (j >> 1) & 1;
-      if (!mbar_wait_bounded(bar(kKEmpty + s), phase ^ 1)) break;
-      c.store_k(smem + T::kK + s * T::kKBytes, t);
-      fence_proxy_async_smem();
-      mbar_arrive(bar(kKFull + s));
-      if (j + 1 < n) c.fetch_k(kc, ks, first + kN, limit, t);
-      if (!mbar_wait_bounded(bar(kVEmpty + s), phase ^ 1)) break;
-      const bool border = first + kN > lowest && lowest < limit;
-      c.store_v(smem + T::kV + s * T::kVBytes, t, border ? s_bad[s] : nullptr);
-      fence_proxy_async_smem();
-      mbar_arrive(bar(kVFull + s));
-      if (j + 1 < n) c.fetch_v(vc, vs, first + kN, limit, t);
+      if (fills_k) {
+        if (!mbar_wait_bounded(bar(kKEmpty + s), phase ^ 1)) break;
+        c.store_k(smem + T::kK + s * T::kKBytes, t);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kKFull + s));
+        if (j + 1 < n) c.fetch_k(kc, ks, first + kN, limit, t);
+      }
+      if (fills_v) {
+        if (!mbar_wait_bounded(bar(kVEmpty + s), phase ^ 1)) break;
+        const bool border = first + kN > lowest && lowest < limit;
+        c.store_v(smem + T::kV + s * T::kVBytes, t, border ? s_bad[s] : nullptr);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kVFull + s));
+        if (j + 1 < n) c.fetch_v(vc, vs, first + kN, limit, t);
+      }
     }
   } else {
     // -------------------------------------------------------------- products
     // By one thread; they run in the order of their issue.
-    if (NQ == 2) give_registers<T::kMmaRegs>();
+    give_registers<T::kMmaRegs>();
     if (warp == kMmaWarp && elect_one()) {
       constexpr uint32_t kShapeS = mma_shape(kM, kN), kShapeO = mma_shape(kM, D);
-      auto scores = [&](int qt, int s) {  // of the keys of stage s
+      auto scores = [&](int qt, int buf, int s) {  // of the keys of stage s
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          tcgen05_mma(tmem + qt * kN, panel_desc(base + T::kQ + qt * T::kQBytes + (k / 4) * (kM * 128) + 32 * (k % 4)),
+          tcgen05_mma(tmem + buf * kN, panel_desc(base + T::kQ + qt * T::kQBytes + (k / 4) * (kM * 128) + 32 * (k % 4)),
                       panel_desc(base + T::kK + s * T::kKBytes + (k / 4) * (kN * 128) + 32 * (k % 4)), kShapeS, k > 0);
-        tcgen05_commit(bar(kSFull + qt));
+        tcgen05_commit(bar(kSFull + buf));
       };
       bool run = n > 0 && mbar_wait_bounded(bar(kKFull), 0);
       if (run) {
         tcgen05_after_sync();
 #pragma unroll
-        for (int qt = 0; qt < NQ; ++qt) scores(qt, 0);
+        for (int qt = 0; qt < NQ; ++qt) scores(qt, qt, 0);
         tcgen05_commit(bar(kKEmpty));
       }
       for (int j = 0; j < n && run; ++j) {
         const int s = j & 1, phase = (j >> 1) & 1;
-        run = mbar_wait_bounded(bar(kVFull + s), phase);
+        if (T::kSBufs == 1) run = mbar_wait_bounded(bar(kVFull + s), phase);
         if (j + 1 < n) run = run && mbar_wait_bounded(bar(kKFull + (s ^ 1)), ((j + 1) >> 1) & 1);
+        if (!run) break;
+        if (T::kSBufs == 2) {
+          if (j + 1 < n) {  // over P of the tile before, which its products have read by then
+            tcgen05_after_sync();
+            scores(0, s ^ 1, s ^ 1);
+            tcgen05_commit(bar(kKEmpty + (s ^ 1)));
+          }
+          run = mbar_wait_bounded(bar(kVFull + s), phase);
+        }
 #pragma unroll
         for (int qt = 0; qt < NQ; ++qt) {
+          const int buf = T::kSBufs == 2 ? s : qt, turn = T::kSBufs == 2 ? phase : j & 1;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            run = run && mbar_wait_bounded(bar((half == 0 ? kPHalf : kPFull) + qt), j & 1);
+            run = run && mbar_wait_bounded(bar((half == 0 ? kPHalf : kPFull) + buf), turn);
             if (!run) break;
             tcgen05_after_sync();
 #pragma unroll
             for (int k = half * (kN / 32); k < (half + 1) * (kN / 32); ++k)
-              tcgen05_mma_ta(tmem + NQ * kN + qt * D, tmem + qt * kN + 8 * k,
+              tcgen05_mma_ta(tmem + T::kOAt + qt * D, tmem + buf * kN + 8 * k,
                              panel_desc(base + T::kV + s * T::kVBytes + (k / 4) * (D * 128) + 32 * (k % 4)), kShapeO,
                              j > 0 || k > 0);
           }
           if (!run) break;
           if (qt == NQ - 1) tcgen05_commit(bar(kVEmpty + s));
-          if (j + 1 < n) {
-            scores(qt, s ^ 1);  // replace P, which the products before them have read by then
-            if (qt == NQ - 1) tcgen05_commit(bar(kKEmpty + (s ^ 1)));
-          } else {
+          if (j + 1 == n) {
             tcgen05_commit(bar(kOFull + qt));
+          } else if (T::kSBufs == 1) {
+            scores(qt, qt, s ^ 1);  // replace P, which the products before them have read by then
+            if (qt == NQ - 1) tcgen05_commit(bar(kKEmpty + (s ^ 1)));
           }
         }
       }
@@ -867,7 +896,7 @@ cudaError_t launch_prefill(const AttnArgs& a, const PrefillShape& p, int64_t lon
     ++split.count;
   if (p.items * split.count > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaError_t e = allow_shared<kv4_prefill_kernel<D, NQ>>(T::kSmem);
-  if (e == cudaSuccess && NQ == 2) e = has_registers<kv4_prefill_kernel<D, NQ>>(T::kLaunchRegs);
+  if (e == cudaSuccess) e = has_registers<kv4_prefill_kernel<D, NQ>>(T::kLaunchRegs);
   if (e != cudaSuccess) return e;
   e = launch_kernel(kv4_prefill_kernel<D, NQ>, p.items * split.count, T::kThreads, T::kSmem, s, a, split, p.blocks_q);
   if (e != cudaSuccess || split.count == 1) return e;
