@@ -50,9 +50,10 @@ __device__ __forceinline__ void cp_async_wait() {
 // over 8192 rows, 1 query row: 87 us against 433; 8 rows: 156 against 452).
 constexpr int64_t kDecodeRows = 8;
 // Query rows of one kv head up to which the decode kernel serves them, in blocks of 8 (12
-// heads of 128, decode kernel against the prompts': 9 rows over 1024 9.8 and 16.9 us, 32
-// rows over 1024 13.6 and 16.6, over 8192 33.9 and 26.0; a batch of 8, 32 rows over
-// 8192 131 and 154).
+// heads of 128, decode kernel against the prompts': 16 rows over 1024 10.1 and 12.2 us, over
+// 8192 20.7 and 24.7, a batch of 8 over 8192 79 and 127; 32 rows 13.6 and 12.1, 38 and
+// 24, 131 and 121: where the two are about even in a batch, its 16 bits of a
+// probability, not 8, decide).
 constexpr int64_t kChunkRows = 32;
 
 // What every attention kernel is given.

@@ -6,9 +6,9 @@
 // tiles of N rows: NQ = 2 and N = 128 up to head_dim 128, 1 and 64 above, where the
 // operands of two stages fill the shared memory.  Three kinds of warps work at once, handing tiles over by
 // mbarriers:
-//   * 4 warps dequantise: codes and scales from global memory (the next tile's are
-//     loaded while this one is converted), bf16 operands to shared memory, two
-//     stages.  k is stored as it lies, [row][element]; v transposed, [element][row],
+//   * 4 warps dequantise (with NQ = 1 4 for k and 4 for v): codes and scales from global
+//     memory (the next tile's are loaded while this one is converted), bf16 operands
+//     to shared memory, two stages.  k is stored as it lies, [row][element]; v transposed, [element][row],
 //     two cache rows' half words put together before the conversion, so that both
 //     operands are K-major.
 //   * 4 warps per query tile do the softmax, a thread per row, the row in registers:
@@ -18,14 +18,17 @@
 //     which neither the bf16 P nor the fp32 sums mind.
 //   * one thread issues the products, S = Q K^T (128 x N, accumulated in tensor memory)
 //     and O += P V with P read from tensor memory: with NQ = 2 those of one query tile
-//     run while the other's softmax does.
+//     run while the other's softmax does, with NQ = 1 S of the next cache tile does.
 // What bounds it: a tile costs 128 exponentials per row on a unit of 16 per clock
 // (2048 cycles for 256 rows), as long as its products on the tensor cores; but a query
 // tile's softmax waits for its own products, P being where S was, so that a tile takes
 // 3400 cycles of softmax and products in turn, the other query tile's in between.
 // Measured (D = 128): 512 queries of 16 heads over 8192 rows 50 us (710 TFLOP/s); 2 x
 // 4096 queries of 12 heads with gate, causal past a prefix of 1000, 125 us (870), and
-// the weights' kernel below 96.
+// the weights' kernel below 96.  With NQ = 1 a tile takes 3300 cycles: the
+// stores of the operands and the products share the shared memory's bandwidth (8 x 64 queries
+// of 12 heads over 8192 rows 121 us; k and v filled by 4 warps in turns 135, with one buffer
+// of S 153; codes loaded two tiles ahead 136).
 // P is rounded to bf16 (2^-8 of itself, the sum l is of the unrounded ones): the
 // operand's type; the error it adds to an output is that of the output's own
 // rounding at most.
