@@ -78,10 +78,10 @@ int64_t attn_rows(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq_len) {
   return num_heads / c->kv_heads * seq_len;
 }
 
-// Bytes of workspace: the scores or the rows' sums that accumulate needs, then
+// Bytes of workspace: the scores and the rows' sums that accumulate needs, then
 // the partial results of a split decode.
 struct AttnBytes {
-  int64_t tracked, parts;
+  int64_t scores, sums, parts;
 };
 
 int check_attention_shape(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq_len, int accumulate, AttnBytes* n) {
@@ -94,9 +94,11 @@ int check_attention_shape(const hrm_kv4_cache* c, int64_t num_heads, int64_t seq
   const int64_t tiles = c->cache_len / 64 + 1;  // of a head; (rows + 7) / 8 blocks of queries walk them
   const int64_t walks = mul_checked(mul_checked(heads, (rows + 7) / 8), tiles);
   if (walks < 0 || walks > INT32_MAX) return HRM_ERR_SIZE_OVERFLOW;
-  const int64_t tracked = mul_checked(mul_checked(all, rows <= hrm::kDecodeRows ? c->cache_len : 1), 4);
-  if (tracked < 0) return HRM_ERR_SIZE_OVERFLOW;
-  n->tracked = accumulate ? (tracked + 15) / 16 * 16 : 0;
+  const int64_t scores = mul_checked(mul_checked(all, c->cache_len), 4);
+  const bool keeps = accumulate && rows <= hrm::kScoreRows;
+  if (keeps && (scores < 0 || scores > INT64_MAX / 2)) return HRM_ERR_SIZE_OVERFLOW;
+  n->scores = keeps ? (scores + 15) / 16 * 16 : 0;
+  n->sums = accumulate && rows > hrm::kDecodeRows ? (all * 4 + 15) / 16 * 16 : 0;
   n->parts = rows <= hrm::kChunkRows ? hrm::kv4_decode_workspace(rows, c->head_dim, c->cache_len)
                                        : hrm::kv4_prefill_workspace(heads, rows, c->head_dim);
   return HRM_OK;
@@ -184,7 +186,7 @@ int hrm_kv4_attention_workspace(const hrm_kv4_cache* cache, int64_t num_heads, i
   AttnBytes w{};
   int e = check_cache_shape(cache, &n);
   if (e == HRM_OK) e = check_attention_shape(cache, num_heads, seq_len, accumulate, &w);
-  if (e == HRM_OK) *bytes = w.tracked + w.parts;
+  if (e == HRM_OK) *bytes = w.scores + w.sums + w.parts;
   return e;
 }
 
@@ -209,9 +211,9 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
     if (accumulate && !cache->weights) return HRM_ERR_NULL_POINTER;
   } else {
     accumulate = 0;  // no row to add to
-    w.tracked = 0;
+    w.scores = w.sums = 0;
   }
-  const int64_t need = w.tracked + w.parts;
+  const int64_t need = w.scores + w.sums + w.parts;
   if (need > 0 && !workspace) return HRM_ERR_NULL_POINTER;
   if (need > 0 && workspace_bytes < need) return HRM_ERR_SCRATCH_LIMIT;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(gate, 16) || (need > 0 && !aligned(workspace, 16)))
@@ -245,13 +247,17 @@ int hrm_kv4_attention(const void* q, const hrm_kv4_cache* cache, const void* gat
   a.prefix_len = prefix_len;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   const int64_t rows = (int64_t)a.group * seq_len;
-  if (accumulate) (rows <= hrm::kDecodeRows ? a.scores : a.lse) = static_cast<float*>(workspace);
+  char* const space = static_cast<char*>(workspace);
+  if (w.scores > 0) a.scores = reinterpret_cast<float*>(space);
+  if (w.sums > 0) a.lse = reinterpret_cast<float*>(space + w.scores);
   const int64_t longest = cache_offsets ? cache->cache_len : cache_offset + seq_len;
-  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.tracked);
+  float* parts = reinterpret_cast<float*>(space + w.scores + w.sums);
   const cudaStream_t s = as_cuda(stream);
   cudaError_t ce = rows <= hrm::kChunkRows ? hrm::launch_kv4_decode(a, cache->head_dim, longest, parts, s)
                                            : hrm::launch_kv4_prefill(a, cache->head_dim, longest, parts, s);
-  if (ce == cudaSuccess && a.lse != nullptr) ce = hrm::launch_kv4_weights(a, cache->head_dim, longest, s);
+  if (ce == cudaSuccess && a.lse != nullptr)
+    ce = a.scores != nullptr ? hrm::launch_kv4_add_weights(a, longest, s)
+                             : hrm::launch_kv4_weights(a, cache->head_dim, longest, s);
   return cuda_status(ce);
 }
 

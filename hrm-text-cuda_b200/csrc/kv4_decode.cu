@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(kClusterWarps * 32, Cta<D, kClusterWarps>::kPe
               e == e0 ? gate0 : (a.gate == nullptr ? 0 : gate_at(a, at)));
   }
   // this CTA's rows, whose scores this CTA wrote
-  if (a.scores != nullptr) add_weights(a, x, t0 * kTileRows, t1 * kTileRows, s.limit, f_m, f_inv);
+  if (a.scores != nullptr && a.lse == nullptr) add_weights(a, x, t0 * kTileRows, t1 * kTileRows, s.limit, f_m, f_inv);
   if (count > 1) cluster.sync();  // the shares are read: no CTA may leave before
 }
 
@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, Cta<D, kShareWarps>::kPerSm)
         const int r = e / (D / 2), d = 2 * (e % (D / 2));
         store_out(a, x, D, r, d, part[r * D + d] * f_inv[r], part[r * D + d + 1] * f_inv[r], s.c_bad[r]);
       }
-      if (a.scores != nullptr) add_weights(a, x, 0, t1 * kTileRows, s.limit, s.c_m, f_inv);
+      if (a.scores != nullptr && a.lse == nullptr) add_weights(a, x, 0, t1 * kTileRows, s.limit, s.c_m, f_inv);
     } else {
       float* mine = part_of(parts, blockIdx.x, pos == begin ? 0 : 1, rows, D);
       for (int e = threadIdx.x; e < x.nrows * D; e += kWarps * 32) mine[e] = part[e];
@@ -902,7 +902,8 @@ __global__ void __launch_bounds__(kJoinThreads, 4) kv4_join_kernel(const AttnArg
     const int item = cuts[side][0].x, c0 = cuts[side][0].y, slot0 = cuts[side][0].z, n = cuts[side][0].w;
     if (item < 0) continue;
     const bool first = c0 == (int)blockIdx.x;  // the item begins here
-    if (!first && a.scores == nullptr) continue;
+    const bool adds = a.scores != nullptr && a.lse == nullptr;
+    if (!first && !adds) continue;
     const Item x = item_of(a, item);
     const float* base = part_of(parts, c0, 0, rows, head_dim);
     auto at = [&](int i) -> const float* { return base + (2 * (int64_t)i + (i == 0 ? slot0 : 0)) * each; };
@@ -977,9 +978,30 @@ __global__ void __launch_bounds__(kJoinThreads, 4) kv4_join_kernel(const AttnArg
         __syncthreads();
       }
     }
-    if (a.scores != nullptr) add_weights(a, x, cuts[side][1].x, cuts[side][1].y, s_limit, f_m, f_inv);
+    if (adds) add_weights(a, x, cuts[side][1].x, cuts[side][1].y, s_limit, f_m, f_inv);
     __syncthreads();
   }
+}
+
+// The probabilities of kDecodeRows to kScoreRows query rows, from the kept scores: a CTA has
+// kAddRows cache rows of a kv head.  Bandwidth: 4 bytes per row and cache row, written and
+// read (16 x 16 heads, 16 query rows over 8192, attention and weights: 214 us; with the
+// scores computed again 528).
+constexpr int kAddRows = 1024, kAddThreads = 256;
+__global__ void __launch_bounds__(kAddThreads) kv4_add_weights_kernel(const AttnArgs a) {
+  __shared__ float s_lse[kScoreRows], s_one[kScoreRows];
+  __shared__ int s_limit[kScoreRows];
+  grid_dependency_begin();
+  const unsigned heads_all = (unsigned)(a.batch * a.kv_heads), chunk = blockIdx.x / heads_all;
+  const int bh = (int)(blockIdx.x - chunk * heads_all), b = bh / a.kv_heads, rows = a.group * a.seq;
+  const Item x{bh, b, bh - b * a.kv_heads, 0, rows};
+  if ((int)threadIdx.x < rows) {
+    s_limit[threadIdx.x] = visible_rows(a, b, (int)(threadIdx.x % (unsigned)a.seq));
+    s_lse[threadIdx.x] = a.lse[((int64_t)b * a.heads + x.hk * a.group) * a.seq + threadIdx.x];
+    s_one[threadIdx.x] = 1.0f;
+  }
+  __syncthreads();
+  add_weights(a, x, (int)chunk * kAddRows, (int)chunk * kAddRows + kAddRows, s_limit, s_lse, s_one);
 }
 
 int64_t items_of(const AttnArgs& a) {
@@ -1033,6 +1055,12 @@ cudaError_t launch_decode(const AttnArgs& a, int64_t longest, float* parts, cuda
 int64_t kv4_decode_workspace(int64_t rows, int64_t head_dim, int64_t longest) {
   if (longest <= kSplitRows) return 0;
   return 2 * shares_for(head_dim) * part_floats(part_rows(rows), head_dim) * (int64_t)sizeof(float);
+}
+
+cudaError_t launch_kv4_add_weights(const AttnArgs& a, int64_t longest, cudaStream_t s) {
+  const int64_t grid = a.batch * a.kv_heads * ((longest + kAddRows - 1) / kAddRows);
+  if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+  return launch_kernel(kv4_add_weights_kernel, grid, kAddThreads, 0, s, a);
 }
 
 cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s) {

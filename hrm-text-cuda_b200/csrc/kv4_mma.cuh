@@ -49,6 +49,9 @@ __device__ __forceinline__ void cp_async_wait() {
 // scores for that; the kernel that computes them again takes longer (16 x 16 heads
 // over 8192 rows, 1 query row: 87 us against 433; 8 rows: 156 against 452).
 constexpr int64_t kDecodeRows = 8;
+// And up to which it keeps the scores, for a kernel that adds several blocks' up:
+// 4 bytes per row and cache row, against the 160 that the cache has of head_dim 128.
+constexpr int64_t kScoreRows = 16;
 // Query rows of one kv head up to which the decode kernel serves them, in blocks of 8 (12
 // heads of 128, decode kernel against the prompts': 16 rows over 1024 10.1 and 12.2 us, over
 // 8192 20.7 and 24.7, a batch of 8 over 8192 79 and 127; 32 rows 13.6 and 12.1, 38 and
@@ -68,8 +71,10 @@ struct AttnArgs {
   const int* cache_offsets;  // per sequence, or null
   int64_t prefix_len;
   float scale_log2;  // softmax scale * log2(e)
-  float* scores;  // weights wanted, rows of one block: [batch * kv_heads, rows, cache_len] scores (log2 units)
-  float* lse;     // weights wanted, more rows: [batch, heads, seq], log2 of each row's sum of 2^score
+  // Weights wanted: up to kScoreRows rows [batch * kv_heads, rows, cache_len] scores (log2
+  // units); past kDecodeRows [batch, heads, seq], log2 of each row's sum of 2^score.
+  float* scores;
+  float* lse;
 };
 
 // Cache rows that the queries of a sequence see: query s rows [0, rows(s)).

@@ -148,6 +148,7 @@ cudaError_t launch_kv4_decode(const AttnArgs& a, int64_t head_dim, int64_t longe
 int64_t kv4_prefill_workspace(int64_t batch_kv_heads, int64_t rows, int64_t head_dim);
 cudaError_t launch_kv4_prefill(const AttnArgs& a, int64_t head_dim, int64_t longest, float* parts, cudaStream_t s);
 cudaError_t kv4_prefill_wait_timeouts(unsigned int* count, bool reset);
+cudaError_t launch_kv4_add_weights(const AttnArgs& a, int64_t longest, cudaStream_t s);
 cudaError_t launch_kv4_weights(const AttnArgs& a, int64_t head_dim, int64_t longest, cudaStream_t s);
 // Whether the selection of `budget` out of at most n rows fits its shared memory.
 bool kv4_evict_fits(int64_t n, int64_t budget);

@@ -123,7 +123,8 @@ def test_attention_workspace_sizes(lib):
 
     assert size(3, 2, 0) == 0
     assert size(3, 2, 1) == 4 * 2 * 3 * 2 * 8       # scores of every query and cache row
-    assert size(6, 5, 1) == 4 * 2 * 6 * 5           # one number per query
+    assert size(6, 5, 1) == 4 * 2 * 6 * 5 * (8 + 1)  # and one number per query
+    assert size(6, 9, 1) == 4 * 2 * 6 * 9           # that alone
     assert size(3, 1, 0, rows=4096) == 0
     assert size(3, 1, 0, rows=65536) > 0            # partial results of a split decode
     assert size(3, 33, 0, rows=65536, batch=200) == 0
