@@ -17,8 +17,9 @@
 // is the threshold are then taken in row order.  When a single row must go (a
 // decode step) it is one CTA-wide minimum instead.
 //
-// Measured: 64 x 16 heads, one of 1025 rows each, 10 us with the write of the new row; 12 heads, 32768 rows to 4096 of D = 128,
-// 28 us; 16 x 16 heads, up to 5000 rows to 1111 of D = 64, 29 us.
+// Measured: 64 x 16 heads, one of 1025 rows each, 10 us with the write of the new row;
+// 12 heads, 32768 rows to 4096 of D = 128, 27 us (a third of it the three digits, a third the
+// copies); 16 x 16 heads, up to 5000 rows to 1111 of D = 64, 28 us.
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
   int* move_at = hole_at + W * steps_at_most;                         // moving rows in the groups before
   int* freed = move_at + W * steps_at_most;                           // in the cluster's first CTA
   __shared__ int buf[2][32];
-  __shared__ int s_totals[3];  // this CTA's rows equal to the threshold, freed places, moving rows
+  __shared__ int s_totals[2];  // this CTA's sums of the counts being ranked
   __shared__ int s_bin, s_above, s_in;
   __shared__ unsigned long long s_low[32];
   __shared__ int2 s_copy[W][kListed];  // (source row, place)
@@ -269,21 +270,30 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
 
   // Ranks in row order: per group a count, then its sum over the groups before, over
   // the CTA (each thread has some consecutive groups) and the cluster's CTAs before.
+  // N kinds of counts at once: their barriers are shared.
   const int groups = W * steps, per_thread = (groups + W * 32 - 1) / (W * 32);
-  auto ranks = [&](int* at, auto count_of, int slot) {
+  auto ranks = [&](auto const& at, auto count_of) {
+    constexpr int N = sizeof(at) / sizeof(at[0]);
     const int g0 = threadIdx.x * per_thread;
-    int mine = 0, all;
-    for (int g = g0; g < g0 + per_thread && g < groups; ++g) mine += count_of(g);
-    int before = cta_scan<W>(mine, buf[slot & 1], &all);
-    if (threadIdx.x == 0) s_totals[slot] = all;
+    int before[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      int mine = 0, all;
+      for (int g = g0; g < g0 + per_thread && g < groups; ++g) mine += count_of(g, x);
+      before[x] = cta_scan<W>(mine, buf[x], &all);
+      if (threadIdx.x == 0) s_totals[x] = all;
+    }
     join();
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (c < rank) before += *cluster.map_shared_rank(&s_totals[slot], c);
-    for (int g = g0; g < g0 + per_thread && g < groups; ++g) {
-      const int n_g = count_of(g);  // (the counts may lie where the ranks go)
-      at[g] = before;
-      before += n_g;
+    for (int x = 0; x < N; ++x) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < rank) before[x] += *cluster.map_shared_rank(&s_totals[x], c);
+      for (int g = g0; g < g0 + per_thread && g < groups; ++g) {
+        const int n_g = count_of(g, x);  // (the counts may lie where the ranks go)
+        at[x][g] = before[x];
+        before[x] += n_g;
+      }
     }
   };
   if (!exact) {  // all digits known: keys equal to the threshold, in row order
@@ -293,10 +303,16 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
       if (lane == 0) hole_at[i * W + warp] = __popc(same);
     }
     __syncthreads();
-    ranks(hole_at, [&](int g) { return hole_at[g]; }, 0);
-    __syncthreads();
+    int* const at[1] = {hole_at};
+    ranks(at, [&](int g, int) { return hole_at[g]; });
+    join();  // the totals are read
   }
 
+  // the bits of group g that are places
+  auto places = [&](int g) -> uint32_t {
+    const int x = kept - (cta_row + 32 * g);
+    return x >= 32 ? kAll : (x <= 0 ? 0u : (1u << x) - 1);
+  };
   // per 32 rows the mask of those that stay
 #pragma unroll
   for (int i = 0; i < steps; ++i) {
@@ -312,15 +328,10 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
     }
     if (lane == 0) masks[i * W + warp] = mask;
   }
-  // the bits of group g that are places
-  auto places = [&](int g) -> uint32_t {
-    const int x = kept - (cta_row + 32 * g);
-    return x >= 32 ? kAll : (x <= 0 ? 0u : (1u << x) - 1);
-  };
   __syncthreads();
   if (n > budget) {
-    ranks(hole_at, [&](int g) { return __popc(~masks[g] & places(g)); }, 1);
-    ranks(move_at, [&](int g) { return __popc(masks[g] & ~places(g)); }, 2);
+    int* const at[2] = {hole_at, move_at};
+    ranks(at, [&](int g, int x) { return __popc(x == 0 ? ~masks[g] & places(g) : masks[g] & ~places(g)); });
     __syncthreads();
     int* list = count == 1 ? freed : cluster.map_shared_rank(freed, 0);
     for (int g = warp; g < groups && places(g) != 0; g += W) {
