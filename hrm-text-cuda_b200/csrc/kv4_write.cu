@@ -10,7 +10,7 @@
 // cos/sin (loaded once) serve every head that it visits.  The gate, q and the
 // rotated k (before quantisation) have the bits of the bf16 prologue.
 //
-// Measured (D = 128, k and v kept): 8 x 4096 tokens of 16 heads 186 us, 0.96 of the
+// Measured (D = 128, k and v kept): 8 x 4096 tokens of 16 heads 187 us, 0.95 of the
 // copy bandwidth; 1001 tokens of 12 heads 8.1 us (4.2 at that bandwidth: one wave of
 // threads that load, shuffle and store once); 64 x 1 tokens 3.4 us, of which an empty
 // launch is 2.
@@ -160,11 +160,13 @@ __global__ void __launch_bounds__(128) kv4_update_kernel(const UpdateArgs a) {
 template <int D>
 cudaError_t launch_split(WriteArgs a, int64_t batch, cudaStream_t s) {
   constexpr int kSlots = Tile<D>::kSlots;
-  // Head slices per tile: all slots for one position, as far as there are heads.  (A
-  // quarter of them, so that a thread's cos/sin serve several heads: 4 x 512 tokens of 16
-  // heads 18.3 against 15.6 us, 64 x 1 7.6 against 3.4.)
+  // Head slices per tile: all slots for one position, as far as there are heads; where the
+  // tiles are many, a quarter of them, so that a thread's cos/sin serve several heads
+  // (16 heads, D = 128, whole against quarter: 64 x 1 tokens 3.4 and 7.6 us, 4 x 512 15.6 and 18.3,
+  // 8 x 4096 with inputs that change from call to call 202 and 190).
   int ht = 1;
   while (ht < kSlots && ht < a.heads) ht *= 2;
+  if (batch * a.seq > 64 * device_sm_count()) ht = ht < 4 ? 1 : ht / 4;
   a.ht = ht;
   const int64_t pt = kSlots / ht;
   a.tiles_per_batch = (a.seq + pt - 1) / pt;
