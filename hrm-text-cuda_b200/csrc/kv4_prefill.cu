@@ -61,6 +61,7 @@ struct Pre {
   // over 8192: 51 us; 168 + 104 + 72: 60; 152 + 120 + 88: 60).
   static constexpr int kLaunchRegs = 128, kSoftmaxRegs = NQ == 2 ? 160 : 184, kFillRegs = 120, kMmaRegs = 72;
   static_assert(NQ * kSoftmaxRegs + (3 - NQ) * kFillRegs + kMmaRegs <= 4 * kLaunchRegs);
+  static_assert(kSoftmaxRegs >= kLaunchRegs && kFillRegs <= kLaunchRegs && kMmaRegs <= kLaunchRegs);  // taken, given
   static constexpr int kQ = 0, kQBytes = kM * D * 2;              // per query tile
   static constexpr int kK = NQ * kQBytes, kKBytes = kN * D * 2;   // per stage
   static constexpr int kV = kK + 2 * kKBytes, kVBytes = D * kN * 2;
