@@ -30,8 +30,8 @@
 //     workspace, and a second launch joins those.
 // The softmax runs online: running maximum and sum in fp32, log2 units.
 //
-// Measured (D = 128): 1 token, 12 heads over 4096 rows 8.6 us, over 65536 38 us (3.3 TB/s
-// of the cache); 32 x 16 heads over up to 8191 rows with gate and weights 111 us (3.3 TB/s).
+// Measured (D = 128): 1 token, 12 heads over 4096 rows 8.6 us, over 65536 39 us (3.2 TB/s
+// of the cache); 32 x 16 heads over up to 8191 rows with gate and weights 96 us (3.8 TB/s).
 // A tile of 32 rows takes a warp 690 to 730 instructions; with 16 x 16 heads over 8192 rows
 // (78 us) the kernel takes 72 us without the copies and 63 without the arithmetic.
 #include <cooperative_groups.h>
@@ -753,18 +753,22 @@ __global__ void __launch_bounds__(kClusterWarps * 32, Cta<D, kClusterWarps>::kPe
 // ---- equal shares of all items' rows, for long caches
 //
 // A sequence has `per` items (kv heads x blocks of query rows) of the same number
-// of 128-row blocks, at least one.  All blocks of all items in order are the
+// of 128-row blocks, and one more for what a piece of work costs beside its rows
+// (32 x 16 heads over up to 8191 rows with weights 96 us; without it, where a share of
+// many short sequences was as long as one of a long one's rows, 111; two: 94, but 83
+// against 82 without weights).  All blocks of all items in order are the
 // positions [0, total); CTA c of G = min(the grid, total) has the positions
 // [total * c / G, total * (c + 1) / G), at least one.
 
 constexpr int kShareRows = kTileRows * kShareWarps;  // rows of a position: a tile per warp
+constexpr int kStart = 1;  // positions that an item's start counts as
 
 struct Line {
   unsigned per, total, shares;
   unsigned mine;  // blocks of the sequence of this lane's number
 };
 __device__ __forceinline__ unsigned blocks_of(const AttnArgs& a, int b) {
-  return max(1, (visible_rows(a, b, a.seq - 1) + kShareRows - 1) / kShareRows);
+  return kStart + (visible_rows(a, b, a.seq - 1) + kShareRows - 1) / kShareRows;
 }
 __device__ __forceinline__ Line line_of(const AttnArgs& a) {  // every lane of the warp
   Line y;
@@ -833,7 +837,8 @@ __global__ void __launch_bounds__(kShareWarps * 32, Cta<D, kShareWarps>::kPerSm)
     const Span span = span_at(a, y, pos);
     const Item x = item_of(a, span.item);
     const unsigned stop = min(end, span.first + span.count);
-    const int t0 = (int)(pos - span.first) * kWarps, t1 = (int)(stop - span.first) * kWarps;
+    const int t0 = max((int)(pos - span.first) - kStart, 0) * kWarps;
+    const int t1 = max((int)(stop - span.first) - kStart, 0) * kWarps;
     attend<D, kWarps, ONE>(a, x, t0, t1, smem, s);
     if (stop - pos == span.count) {  // the whole item
       if (threadIdx.x < x.nrows) {

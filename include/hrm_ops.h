@@ -364,8 +364,8 @@ int hrm_kv4_evict(const hrm_kv4_cache* cache, const hrm_kv4_cache* out, int64_t 
 
 /* Number of bounded device-side waits that ran out on the current device
  * since the library was loaded there (or since the last reset).  The
- * bulk-copy kernels of the opt-in build and hrm_kv4_attention for more than 32
- * query rows of a kv head wait on mbarriers with a deadline of
+ * bulk-copy kernels of the opt-in build, and hrm_kv4_attention for more than 32
+ * query rows of a kv head (16 with accumulate), wait on mbarriers with a deadline of
  * about one second; a wait that runs out counts itself here and the kernel
  * returns instead of hanging, leaving the affected rows unwritten.  It reads
  * device memory: call it after synchronizing the streams that ran the
