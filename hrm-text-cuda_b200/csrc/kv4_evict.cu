@@ -18,7 +18,7 @@
 // decode step) it is one CTA-wide minimum instead.
 //
 // Measured: 64 x 16 heads, one of 1025 rows each, 10 us with the write of the new row;
-// 12 heads, 32768 rows to 4096 of D = 128, 27 us (a third of it the three digits, a third the
+// 12 heads, 32768 rows to 4096 of D = 128, 25 us (a third of it the three digits, a third the
 // copies); 16 x 16 heads, up to 5000 rows to 1111 of D = 64, 28 us.
 #include <cooperative_groups.h>
 
@@ -345,6 +345,13 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
   // Copies: each warp its rows that stay (in place: that move).  They are listed until
   // the list could overflow, so that many rows' reads are in flight at once.
   const int per_pass = 32 / lanes, part = lane / lanes;
+  // Weight and position go with the row's codes, by its first two lanes, in clusters of CTAs of
+  // 2048 to 4096 rows, else before them, a lane per row (12 heads, 32768 rows on 8
+  // CTAs 25.0 against 27.2 us; 8192 on 4 18.4 and 17.7; 16 x 16 heads of 5000 on one
+  // CTA, whose keys leave no registers for it, 29.9 and 28.0).
+  const bool with_codes = W == 16 && K == 8 && count > 1;
+  const uint32_t* word_from = reinterpret_cast<const uint32_t*>(sub == 0 ? (const void*)weights : positions);
+  uint32_t* word_to = reinterpret_cast<uint32_t*>(sub == 0 ? (void*)(a.to.weights + to0) : a.to.positions + to0);
   constexpr int kAhead = 4;
   int listed = 0;
   for (int i = 0; i < steps; ++i) {
@@ -360,7 +367,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
     listed += __popc(todo);
     if (listed <= kListed - 32 && i + 1 < steps) continue;
     __syncwarp();
-    for (int r = lane; r < listed; r += 32) {
+    for (int r = lane; !with_codes && r < listed; r += 32) {
       const int2 c = s_copy[warp][r];
       const float w = weights[c.x];
       const int at = positions[c.x];
@@ -369,7 +376,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
     }
     for (int r0 = part; r0 < listed; r0 += kAhead * per_pass) {
       uint4 code[kAhead];
-      uint32_t scale[kAhead];
+      uint32_t scale[kAhead], word[kAhead];
       int to[kAhead];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
@@ -379,6 +386,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
         if (works) {  // past the last row: the first once more
           code[x] = code_from[(int64_t)c.x * p];
           scale[x] = scale_from[(int64_t)c.x * p];
+          if (with_codes && sub < 2) word[x] = word_from[c.x];
         }
       }
 #pragma unroll
@@ -386,6 +394,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
         if (to[x] >= 0) {
           code_to[(int64_t)to[x] * p] = code[x];
           scale_to[(int64_t)to[x] * p] = scale[x];
+          if (with_codes && sub < 2) word_to[to[x]] = word[x];
         }
     }
     __syncwarp();
