@@ -439,13 +439,18 @@ cudaError_t launch_kv4_evict(const Kv4View& from, const Kv4View& to, bool in_pla
   const int64_t n = lengths ? from.cache_len : (length < from.cache_len ? length : from.cache_len);
   // CTAs per head: while they leave room on the GPU (2 of 512 threads per SM) and have 2048 rows
   // each (12 heads: 2048 rows on one CTA 11.4 us, on two 15.8; 4096 17.3 and 18.0; 8192 25.6
-  // and, on four, 18.0; 32768 198 and, on eight, 27.7)
+  // and, on four, 18.0; 32768 198 and, on eight, 27.7); also without that room, where a
+  // CTA's keys would not fit its registers (256 heads of 12000 rows, D = 64: on one 166 us,
+  // on two 128; 128 of 20000: on two 137, on four 126).
+  constexpr int64_t kKeys = 16 * 512;  // keys that a CTA holds at most
   int count = 1;
-  while (count < 8 && batch * kv_heads * count * 2 <= 2 * device_sm_count() && n >= 2048 * count * 2) count *= 2;
+  while (count < 8 && n >= 2048 * count * 2 &&
+         (batch * kv_heads * count * 2 <= 2 * device_sm_count() || n > kKeys * count))
+    count *= 2;
   const int64_t mine = (n + count - 1) / count;
   if (mine <= 8 * 256) return launch<8, 8>(a, batch, n, count, s);
   if (mine <= 8 * 512) return launch<16, 8>(a, batch, n, count, s);
-  if (mine <= 16 * 512) return launch<16, 16>(a, batch, n, count, s);
+  if (mine <= kKeys) return launch<16, 16>(a, batch, n, count, s);
   return launch<16, 0>(a, batch, n, count, s);
 }
 

@@ -179,6 +179,15 @@ def step(c, gqkv, heads, rows, position, budget, protect, theta=10000.0):
     return ops.kv4_attention(q, c, rows, gate=gate, accumulate=True)
 
 
+@pytest.mark.parametrize("place", ["in place", "out"])
+def test_evict_long_rows_of_many_heads(cuda, place):
+    """More clusters than the GPU holds at once."""
+    c = filled(19, 8, 8500, 64, 70)
+    lengths = [8500 - 400 * i for i in range(19)]
+    out = ops.kv4_cache(19, 8, 3000, 64, track=True) if place == "out" else None
+    base.check_evict(c, lengths, 3000, 8000, out)
+
+
 def test_two_streams_at_once(cuda):
     """Two servers' steps side by side: each as if it ran alone."""
     h, d, b = 4, 128, 3
