@@ -10,6 +10,10 @@ A decode loop with a bounded cache, one step:
 
 Offsets and lengths are ints, or int32 CUDA tensors with one value per sequence
 (read on the device, so that a captured step can be replayed as they advance).
+
+With `stream` a call is queued there, and the tensors that it makes belong to that
+stream, as torch's own do under `with torch.cuda.stream(stream)`: another stream that
+uses them waits for it first and, before it drops them, calls record_stream.
 """
 
 from __future__ import annotations
@@ -22,7 +26,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._lib import HRM_OK, LIB, Kv4CacheStruct, check
-from .ops import _need
+from .ops import _need, _on
 
 GROUP = 32  # elements per (scale, base) pair
 HEAD_DIMS = (64, 128, 192, 256)
@@ -165,8 +169,9 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
     s = gqkv.shape[1]
     if out is None:
-        gate, q = gqkv.new_empty((b, s, h, d)), gqkv.new_empty((b, h, s, d))
-        k, v = (torch.empty_like(q), torch.empty_like(q)) if keep_kv else (None, None)
+        with _on(stream):
+            gate, q = gqkv.new_empty((b, s, h, d)), gqkv.new_empty((b, h, s, d))
+            k, v = (torch.empty_like(q), torch.empty_like(q)) if keep_kv else (None, None)
         given = ()
     else:
         gate, q, k, v = given = tuple(out)
@@ -214,7 +219,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
         if gate.numel() != q.numel():
             raise ValueError("gate has the wrong size")
     if out is None:
-        out = q.new_empty((b, s, h, d))
+        with _on(stream):
+            out = q.new_empty((b, s, h, d))
     else:
         _need(out, "out")
         if out.numel() != q.numel():
@@ -224,11 +230,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
         raise ValueError("accumulate needs a cache with weights (kv4_cache(..., track=True))")
     nbytes = kv4_attention_workspace(cache, h, s, accumulate)
     if nbytes and workspace is None:
-        if stream is None:
+        with _on(stream):
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        else:  # on the launch's stream, so that the allocator reuses it in that stream's order
-            with torch.cuda.stream(stream):
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     elif workspace is not None:
         _need(workspace, "workspace", (torch.uint8,))
         nbytes = workspace.numel()
@@ -269,7 +272,8 @@ def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offse
     length, length_t = _offset(lengths, "lengths", b)
     protect, protect_t = _offset(protect_from, "protect_from", b)
     if new_lengths is None:
-        new_lengths = cache.positions.new_empty(b)
+        with _on(stream):
+            new_lengths = cache.positions.new_empty(b)
     else:
         _need(new_lengths, "new_lengths", (torch.int32,))
         if new_lengths.numel() != b:

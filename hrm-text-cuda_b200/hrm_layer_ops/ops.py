@@ -10,6 +10,7 @@ stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -27,6 +28,15 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[ctypes.c_void_p]:
 def _stream(t: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> ctypes.c_void_p:
     s = stream if stream is not None else torch.cuda.current_stream(t.device)
     return _vp(s.cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(stream: Optional[torch.cuda.Stream]):
+    """Allocations for a launch on `stream` come from that stream's pool: a block of the
+    current stream's may be in use by kernels that are still queued there."""
+    return _HERE if stream is None else torch.cuda.stream(stream)
 
 
 def _launch(name: str, tensors, stream: Optional[torch.cuda.Stream], *args) -> None:
