@@ -5,7 +5,9 @@ libhrm_ops.so.  Inputs must be contiguous CUDA tensors, all on one device; a
 CPU tensor, or a tensor on another GPU, is an error, never a silent fallback.
 The launch runs with that device current (the library sizes its grids from
 the current device and launches there), by default on its current torch
-stream.
+stream.  With `stream`, the tensors that a call makes belong to that stream,
+as torch's own do under `with torch.cuda.stream(stream)`: another stream that
+uses them waits for it first and, before it drops them, calls record_stream.
 """
 
 from __future__ import annotations
@@ -79,7 +81,9 @@ def additive_inject(z_a: torch.Tensor, z_b: torch.Tensor, out: Optional[torch.Te
     _need(z_a, "z_a"); _need(z_b, "z_b")
     if z_a.numel() != z_b.numel():
         raise ValueError("z_a and z_b differ in size")
-    out = torch.empty_like(z_a) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty_like(z_a)
     _need(out, "out")
     if out.numel() != z_a.numel():
         raise ValueError("out has the wrong size")
@@ -93,7 +97,9 @@ def swiglu_ffn(gate: torch.Tensor, up: torch.Tensor, out: Optional[torch.Tensor]
     _need(gate, "gate"); _need(up, "up")
     if gate.numel() != up.numel():
         raise ValueError("gate and up differ in size")
-    out = torch.empty_like(gate) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty_like(gate)
     _need(out, "out")
     if out.numel() != gate.numel():
         raise ValueError("out has the wrong size")
@@ -118,7 +124,9 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
         _need(weight, "weight", (x.dtype,))
         if weight.numel() != hidden:
             raise ValueError("weight must have hidden_size elements")
-    out = torch.empty_like(x) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty_like(x)
     _need(out, "out", (x.dtype,))
     if out.numel() != x.numel():
         raise ValueError("out has the wrong size")
@@ -142,8 +150,12 @@ def add_rms_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.T
         _need(weight, "weight")
         if weight.numel() != hidden:
             raise ValueError("weight must have hidden_size elements")
-    residual_out = torch.empty_like(x) if residual_out is None else residual_out
-    normed_out = torch.empty_like(x) if normed_out is None else normed_out
+    if residual_out is None:
+        with _on(stream):
+            residual_out = torch.empty_like(x)
+    if normed_out is None:
+        with _on(stream):
+            normed_out = torch.empty_like(x)
     _need(residual_out, "residual_out"); _need(normed_out, "normed_out")
     if residual_out.numel() != x.numel() or normed_out.numel() != x.numel():
         raise ValueError("outputs have the wrong size")
@@ -158,7 +170,8 @@ def rope_table(max_positions: int, head_dim: int, theta: float = 10000.0,
     """fp32 [max_positions, head_dim] table: cos in [:, :hd/2], sin in [:, hd/2:]."""
     if out is None:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        out = torch.empty((max_positions, head_dim), dtype=torch.float32, device=device)
+        with _on(stream):
+            out = torch.empty((max_positions, head_dim), dtype=torch.float32, device=device)
     _need(out, "out", (torch.float32,))
     if out.numel() != max_positions * head_dim:
         raise ValueError("out has the wrong size")
@@ -213,7 +226,9 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, embedding_scale: fl
     if table.dim() != 2:
         raise ValueError("table must be [vocab, hidden]")
     vocab, hidden = table.shape
-    out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=table.device) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=table.device)
     _need(out, "out")
     if out.numel() != ids.numel() * hidden:
         raise ValueError("out has the wrong size")
@@ -234,8 +249,11 @@ def embed_rms_norm(ids: torch.Tensor, table: torch.Tensor, embedding_scale: floa
     vocab, hidden = table.shape
     shape = (*ids.shape, hidden)
     if hidden_out is None and keep_hidden:
-        hidden_out = torch.empty(shape, dtype=table.dtype, device=table.device)
-    normed_out = torch.empty(shape, dtype=table.dtype, device=table.device) if normed_out is None else normed_out
+        with _on(stream):
+            hidden_out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    if normed_out is None:
+        with _on(stream):
+            normed_out = torch.empty(shape, dtype=table.dtype, device=table.device)
     if hidden_out is not None:
         _need(hidden_out, "hidden_out")
     _need(normed_out, "normed_out")
@@ -264,8 +282,9 @@ def split_gqkv_rope(gqkv: torch.Tensor, num_heads: int, position_offset: int = 0
     b, s, w = gqkv.shape
     d = w // (4 * num_heads)
     if out is None:
-        out = (torch.empty((b, s, num_heads, d), dtype=gqkv.dtype, device=gqkv.device),
-               *(torch.empty((b, num_heads, s, d), dtype=gqkv.dtype, device=gqkv.device) for _ in range(3)))
+        with _on(stream):
+            out = (torch.empty((b, s, num_heads, d), dtype=gqkv.dtype, device=gqkv.device),
+                   *(torch.empty((b, num_heads, s, d), dtype=gqkv.dtype, device=gqkv.device) for _ in range(3)))
     for t, n in zip(out, ("gate", "q", "k", "v")):
         _need(t, n)
     positions, cache_len = 0, 0
@@ -291,7 +310,9 @@ def gated_attn_output(gate: torch.Tensor, attn_out: torch.Tensor, out: Optional[
     _need(gate, "gate"); _need(attn_out, "attn_out")
     if gate.numel() != attn_out.numel():
         raise ValueError("gate and attn_out differ in size")
-    out = torch.empty_like(attn_out) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty_like(attn_out)
     _need(out, "out")
     _launch("hrm_gated_attn_output", (gate, attn_out, out), stream, _ptr(gate), _ptr(attn_out), _ptr(out),
             gate.numel())
@@ -311,7 +332,9 @@ def broadcast_vec(src: torch.Tensor, n_copies: int, out: Optional[torch.Tensor] 
                   stream=None) -> torch.Tensor:
     """out[r, :] = src for r < n_copies (bf16).  src/lib.rs:748-767."""
     _need(src, "src")
-    out = torch.empty((n_copies, src.numel()), dtype=src.dtype, device=src.device) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty((n_copies, src.numel()), dtype=src.dtype, device=src.device)
     _need(out, "out")
     if out.numel() != n_copies * src.numel():
         raise ValueError("out has the wrong size")
@@ -330,7 +353,9 @@ def convert_to_bf16(raw: torch.Tensor, dtype: str, out: Optional[torch.Tensor] =
     if raw.numel() % size:
         raise ValueError("raw byte count is not a multiple of the element size")
     n = raw.numel() // size
-    out = torch.empty(n, dtype=torch.bfloat16, device=raw.device) if out is None else out
+    if out is None:
+        with _on(stream):
+            out = torch.empty(n, dtype=torch.bfloat16, device=raw.device)
     _need(out, "out")
     if out.numel() != n:
         raise ValueError("out has the wrong size")
