@@ -310,7 +310,10 @@ def _upload(path, chunks, device, chunk_bytes, reader_threads, stream):
     staging_bytes = min(cap, 32 << 20) // 16 * 16 or 16
     staging = torch.empty(staging_bytes, dtype=torch.uint8, device=device)
     events: List[Optional[torch.cuda.Event]] = [None] * len(host)
-    s = stream if stream is not None else torch.cuda.current_stream(device)
+    s = torch.cuda.current_stream(device)
+    if stream is not None:  # kernels queued here may still use what the weights' blocks held before
+        stream.wait_stream(s)
+        s = stream
     fd = os.open(path, os.O_RDONLY)
     try:
         with ThreadPoolExecutor(max_workers=max(1, reader_threads)) as pool, torch.cuda.device(device):
