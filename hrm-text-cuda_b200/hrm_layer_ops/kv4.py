@@ -66,7 +66,7 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class Kv4Cache:
     """The buffers of one 4-bit cache (one layer's KV slot).
 
@@ -76,7 +76,8 @@ class Kv4Cache:
     positions          int32 [batch, kv_heads, cache_len], or None
 
     The shapes are checked here, once; the calls then pass the buffers as they
-    are.  Do not resize or replace the tensors of a cache: make another one.
+    are.  A cache's tensors cannot be replaced (make another one) and must not be
+    resized; write into them to reset them.
     """
 
     k_codes: torch.Tensor
@@ -92,7 +93,8 @@ class Kv4Cache:
         if self.k_codes.dim() != 4 or 2 * self.k_codes.shape[3] not in HEAD_DIMS:
             raise ValueError("k_codes must be [batch, kv_heads, cache_len, head_dim / 2], head_dim 64, 128, 192 or 256")
         b, h, n, half = self.k_codes.shape
-        self.shape = (b, h, n, 2 * half)
+        put = object.__setattr__  # (frozen: the struct below holds these tensors' addresses)
+        put(self, "shape", (b, h, n, 2 * half))
         want = {"v_codes": ((b, h, n, half), torch.uint8), "k_scales": ((b, h, n, 2 * half // GROUP, 2), torch.bfloat16),
                 "v_scales": ((b, h, n, 2 * half // GROUP, 2), torch.bfloat16), "weights": ((b, h, n), torch.float32),
                 "positions": ((b, h, n), torch.int32)}
@@ -107,10 +109,10 @@ class Kv4Cache:
                 raise ValueError(f"{name} is on {t.device}, k_codes on {self.k_codes.device}")
         ptr = [None if t is None else t.data_ptr()
                for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.weights, self.positions)]
-        self._struct = Kv4CacheStruct(*ptr, b, h, n, 2 * half)
-        self._ref = ctypes.pointer(self._struct)
-        self.device = self.k_codes.device
-        self._workspaces = {}  # bytes by (heads, seq, accumulate)
+        put(self, "_struct", Kv4CacheStruct(*ptr, b, h, n, 2 * half))
+        put(self, "_ref", ctypes.pointer(self._struct))
+        put(self, "device", self.k_codes.device)
+        put(self, "_workspaces", {})  # bytes by (heads, seq, accumulate)
 
 
 def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, device=None, track: bool = False) -> Kv4Cache:
