@@ -12,7 +12,7 @@
 // (hi - lo) / 15; the roundings of S and Z to 8 significant bits move the grid by
 // at most 2^-8 of (hi - lo) and 2^-8 of |lo - S| (a tenth of a step for values
 // around zero), and n is taken against the rounded grid.  A group that holds a NaN or an infinity, or whose
-// S or Z is out of bf16's range, gets S = NaN and reads back as NaN.
+// S, Z or largest value S * 31/16 + Z is out of bf16's range, gets S = NaN and reads back as NaN.
 //
 // Why 1 + n/16 and not n: the bf16 pattern 0x3f80 | n << 3 IS 1 + n/16, so a
 // code becomes a bf16 operand with one shift and one and-or (two elements at
@@ -57,6 +57,13 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
 __device__ __forceinline__ uint32_t kv4_scale2(uint32_t sz) { return __byte_perm(sz, sz, 0x1010); }
 __device__ __forceinline__ uint32_t kv4_base2(uint32_t sz) { return __byte_perm(sz, sz, 0x3232); }
 
+// A word (S, Z) some of whose 16 values are not finite: those lie between S + Z and
+// S * 31/16 + Z, which is a NaN or an infinity where S or Z is.
+__device__ __forceinline__ bool kv4_not_finite(uint32_t sz) {
+  const uint32_t x = fma_bf16x2(0x3ff83f80u, kv4_scale2(sz), kv4_base2(sz));
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
 // 1 + n/16 of nibbles P and P + 4 of w, as a packed bf16 pair: one shift and one
 // three-input and-or (written out: the compiler made two instructions of it).
 // Extracting nibbles 0 and 1 without a shift, by packed fmas that scale the masked
@@ -96,11 +103,11 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint4& x, uint32_t quad, 
   const float scale = bf16_to_f32((uint16_t)s);
   const uint32_t z = f32_to_bf16(__fsub_rn(lo, scale));
   const float base = bf16_to_f32((uint16_t)z);
-  if (!(fabsf(scale) < INFINITY) || !(fabsf(base) < INFINITY)) {
+  sz = s | z << 16;
+  if (kv4_not_finite(sz)) {
     sz = 0x00007fc0u;  // S = NaN, Z = 0
     return 0;
   }
-  sz = s | z << 16;
   if (s == 0) return 0;
   const float inv = __fdiv_rn(16.0f, scale);
   uint32_t codes = 0;

@@ -93,9 +93,4 @@ struct Visible {
 };
 __device__ __forceinline__ int visible_rows(const AttnArgs& a, int b, int s) { return Visible(a, b).rows(s); }
 
-// A word (S, Z) whose group reads back as NaN or an infinity.
-__device__ __forceinline__ bool kv4_not_finite(uint32_t sz) {
-  return (sz & 0x7f80u) == 0x7f80u || (sz & 0x7f800000u) == 0x7f800000u;
-}
-
 }  // namespace hrm

@@ -273,11 +273,13 @@ int hrm_upload_to_bf16_static(const void* src, int src_dtype, void* dst, int64_t
  *   S = bf16_rn((hi - lo) * (16/15)), 0 where hi - lo < 2^-100
  *   Z = bf16_rn(lo - S)
  *   code = clamp(rint((x - Z) * (16 / S) - 16), 0, 15), 0 where S == 0;
- * a group that holds a NaN or an infinity, or whose S or Z overflows bf16,
- * reads back as NaN.  All buffers are row-major [batch, kv_heads, cache_len, ...];
- * codes and scales are 16-byte aligned (HRM_ERR_ALIGNMENT otherwise, also for
- * the 16-bit tensors of these calls).  A row is 5 bits per element: 160 bytes
- * for k and v of head_dim 128, against 512 in bf16.  No reference counterpart
+ * a group that holds a NaN or an infinity, or whose S, Z or S * 31/16 + Z overflows
+ * bf16, reads back as NaN.  (In codes and scales from elsewhere, a group whose
+ * S + Z or S * 31/16 + Z is not finite may count as NaN as a whole.)  All buffers
+ * are row-major [batch, kv_heads, cache_len, ...]; codes and scales are 16-byte
+ * aligned (HRM_ERR_ALIGNMENT otherwise, also for the 16-bit tensors of these
+ * calls).  A row is 5 bits per element: 160 bytes for k and v of head_dim 128,
+ * against 512 in bf16.  No reference counterpart
  * (its cache is bf16, src/kernels/kv_cache_update.cu:12-48).
  *
  * Offsets come as one host value or, where the array is not NULL, as one int32
