@@ -73,8 +73,17 @@ struct Pre {
   static constexpr uint32_t kColumns = tmem_columns(kOAt + NQ * D);  // S of each tile, then O of each
 };
 
-// Barriers, in order: pairs by stage; S and P by query tile, or by buffer of S; O by query tile.
-enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPHalf = 10, kPFull = 12, kOFull = 14, kBars = 16 };
+// Barriers, in order: pairs by stage; S and P by query tile, or by buffer of S; O by query tile;
+// the last products, where a wait ran out.
+enum {
+  kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPHalf = 10, kPFull = 12, kOFull = 14, kDone = 16,
+  kBars = 17
+};
+
+// What is left by rows whose waits ran out: in a partial result's mask of groups this bit,
+// so that the joining kernel does not write them; as the log of their sum +inf, so
+// that the weights' kernel finds all their probabilities 0.
+constexpr uint32_t kTimedOut = 1u << 31;
 
 struct PrefillSplit {
   int count;     // CTAs per item (kv head x block of query rows)
@@ -265,6 +274,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         mbar_init(bar(kPFull + i), kM);
         mbar_init(bar(kOFull + i), 1);
       }
+      mbar_init(bar(kDone), 1);
       mbar_init_fence();
     }
     __syncwarp();
@@ -385,6 +395,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       const uint64_t both = add_f32x2(sum[0], sum[1]);
       l += lo_f32(both) + hi_f32(both);
     }
+    if (!ok) tmem_wait_store();
     const unsigned row = row0 + r;
     const unsigned g = row / a.seq, sq = row - g * a.seq;
     const int64_t head = hk * a.group + g;
@@ -414,7 +425,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
     if (split.count == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (row < rows && a.lse != nullptr)
-        a.lse[q_row0() + row] = m == -INFINITY ? -INFINITY : m * scale + log2f(l);
+        a.lse[q_row0() + row] = !ok ? INFINITY : (m == -INFINITY ? -INFINITY : m * scale + log2f(l));
       cp_async_wait_all();
       __syncwarp();
 #pragma unroll 1
@@ -465,7 +476,7 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       float* tail = part + NQ * kM * D + r;
       tail[0] = m == -INFINITY ? -INFINITY : m * scale;  // log2 units
       tail[NQ * kM] = l;
-      tail[2 * NQ * kM] = __uint_as_float(bad);
+      tail[2 * NQ * kM] = __uint_as_float(ok ? bad : kTimedOut);
     }
   } else if (fills) {
     // --------------------------------------------------------------- filling
@@ -557,6 +568,10 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
           }
         }
       }
+      if (n > 0 && !run) {  // a wait ran out: what was issued ends before its memory is given back
+        tcgen05_commit(bar(kDone));
+        mbar_wait_bounded(bar(kDone), 0);
+      }
     }
   }
   __syncwarp();
@@ -617,10 +632,13 @@ __global__ void __launch_bounds__(kM) kv4_prefill_join_kernel(const AttnArgs a, 
     }
     top = now;
   }
+  const bool timed_out = bad & kTimedOut;
   const unsigned g = row / a.seq, s = row - g * a.seq;
   const int64_t head = hk * a.group + g;
   if (a.lse != nullptr && d0 == 0)
-    a.lse[((int64_t)b * a.heads + hk * a.group) * a.seq + row] = top == -INFINITY ? -INFINITY : top + log2f(norm);
+    a.lse[((int64_t)b * a.heads + hk * a.group) * a.seq + row] =
+        timed_out ? INFINITY : (top == -INFINITY ? -INFINITY : top + log2f(norm));
+  if (timed_out) return;  // unwritten, as without a split
   const float inv = norm == 0.0f ? 0.0f : 1.0f / norm;
   const bool nan = bad >> (d0 / kKv4Group) & 1u;
   const int64_t at = (((int64_t)b * a.seq + s) * a.heads + head) * D + d0;
@@ -660,7 +678,7 @@ struct Wgt {
   static constexpr int kThreads = 128 + 128 + 32;
   static constexpr uint32_t kColumns = 256;
 };
-enum { kWFull = 0, kWEmpty = 2, kWSFull = 4, kWSEmpty = 6, kWBars = 8 };
+enum { kWFull = 0, kWEmpty = 2, kWSFull = 4, kWSEmpty = 6, kWDone = 8, kWBars = 9 };
 
 // The query tiles of a kv head with a row that sees cache row `first` or one after it,
 // in order.  (Asking each tile in turn for its limits, divisions and all, took 750
@@ -743,6 +761,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
         mbar_init(bar(kWSFull + i), 1);
         mbar_init(bar(kWSEmpty + i), 128);
       }
+      mbar_init(bar(kWDone), 1);
       mbar_init_fence();
     }
     __syncwarp();
@@ -762,10 +781,12 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     float extra = 0.0f;  // of tiles with masked probabilities
     const uint64_t scale2 = pack_f32x2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
     int n = 0, more = 1;  // (`first` < limit: there is a tile)
+    bool ok = true;
     while (more) {
       const int s = n & 1, phase = (n >> 1) & 1, entry = n & 3;
       ++n;
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(kWSFull + s), phase))) break;
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kWSFull + s), phase));
+      if (!ok) break;
       tcgen05_after_sync();
       const bool whole = s_whole[entry] != 0;
       more = s_more[entry];
@@ -798,7 +819,7 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
       mbar_arrive(bar(kWSEmpty + s));
     }
     const uint64_t both = add_f32x2(sum[0], sum[1]);
-    if (at < limit) a.c.weights[head_row + at] += lo_f32(both) + hi_f32(both) + extra;
+    if (ok && at < limit) a.c.weights[head_row + at] += lo_f32(both) + hi_f32(both) + extra;
   } else if (warp < 8) {
     // ----------------------------------------------------------------- queries
     const int t = tid - 128;
@@ -843,9 +864,11 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
     // ---------------------------------------------------------------- products
     constexpr uint32_t kShape = mma_shape(128, 128);
     int n = 0, more = 1;
+    bool run = true;
     while (more) {
       const int s = n & 1, phase = (n >> 1) & 1;
-      if (!mbar_wait_bounded(bar(kWFull + s), phase) || !mbar_wait_bounded(bar(kWSEmpty + s), phase ^ 1)) break;
+      run = mbar_wait_bounded(bar(kWFull + s), phase) && mbar_wait_bounded(bar(kWSEmpty + s), phase ^ 1);
+      if (!run) break;
       more = s_more[n++ & 3];
       tcgen05_after_sync();
 #pragma unroll
@@ -856,6 +879,10 @@ __global__ void __launch_bounds__(Wgt<D>::kThreads) kv4_weights_kernel(const Att
       }
       tcgen05_commit(bar(kWSFull + s));
       tcgen05_commit(bar(kWEmpty + s));
+    }
+    if (!run) {  // as in the attention's kernel
+      tcgen05_commit(bar(kWDone));
+      mbar_wait_bounded(bar(kWDone), 0);
     }
   }
   __syncwarp();

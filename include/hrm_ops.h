@@ -369,8 +369,10 @@ int hrm_kv4_evict(const hrm_kv4_cache* cache, const hrm_kv4_cache* out, int64_t 
  * bulk-copy kernels of the opt-in build, and hrm_kv4_attention for more than 32
  * query rows of a kv head (16 with accumulate), wait on mbarriers with a deadline of
  * about one second; a wait that runs out counts itself here and the kernel
- * returns instead of hanging, leaving the affected rows unwritten.  It reads
- * device memory: call it after synchronizing the streams that ran the
+ * returns instead of hanging, leaving the affected rows unwritten (of an attention
+ * that accumulates: its output's rows, whose probabilities no weight gets, or the
+ * weights of some cache rows as they were).  It reads device memory: call it
+ * after synchronizing the streams that ran the
  * library's kernels.  0 in correct operation.  reset != 0 sets the count back to 0 after
  * reading it.  No reference counterpart (the reference's kernels have no
  * waits).                                                                   */
