@@ -542,15 +542,21 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& x, int t0,
       // finite: 0 * NaN would reach them.  Such groups are read as zeros here and
       // the queries that do see them are marked.
       if (border && lowest < limit) {
-        for (int r = 0; r < kTileRows; ++r) {
-          uint32_t* vs = reinterpret_cast<uint32_t*>(st + kVScales);
-          const bool mine = lane < T::kGroups && kv4_not_finite(vs[r * T::kGroups + lane]);
-          const uint32_t found = __ballot_sync(kAll, mine);
-          if (mine) vs[r * T::kGroups + lane] = 0;
-          if (first + r < my_limit[0]) bad[0] |= found;
-          if (first + r < my_limit[1]) bad[1] |= found;
+        uint32_t* vs = reinterpret_cast<uint32_t*>(st + kVScales);
+        bool any = false;  // in this lane's row
+#pragma unroll
+        for (int x = 0; x < T::kGroups; ++x) any |= kv4_not_finite(vs[lane * T::kGroups + x]);
+        if (__any_sync(kAll, any)) {
+#pragma unroll 1
+          for (int r = 0; r < kTileRows; ++r) {
+            const bool mine = lane < T::kGroups && kv4_not_finite(vs[r * T::kGroups + lane]);
+            const uint32_t found = __ballot_sync(kAll, mine);
+            if (mine) vs[r * T::kGroups + lane] = 0;
+            if (first + r < my_limit[0]) bad[0] |= found;
+            if (first + r < my_limit[1]) bad[1] |= found;
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
     }
 
