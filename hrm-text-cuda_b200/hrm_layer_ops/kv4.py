@@ -26,7 +26,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._lib import HRM_OK, LIB, Kv4CacheStruct, check
-from .ops import _need, _on
+from .ops import _made, _need
 
 GROUP = 32  # elements per (scale, base) pair
 HEAD_DIMS = (64, 128, 192, 256)
@@ -157,6 +157,11 @@ def kv4_update(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, position_offse
     return cache
 
 
+def _split_results(gqkv: torch.Tensor, b: int, s: int, h: int, d: int, keep_kv: bool):
+    gate, q = gqkv.new_empty((b, s, h, d)), gqkv.new_empty((b, h, s, d))
+    return (gate, q, torch.empty_like(q), torch.empty_like(q)) if keep_kv else (gate, q, None, None)
+
+
 def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, position_offset: Offset = 0,
                         theta: float = 10000.0, table: Optional[torch.Tensor] = None, cache_offset: Offset = 0,
                         out=None, keep_kv: bool = True, *, stream=None):
@@ -171,9 +176,7 @@ def split_gqkv_rope_kv4(gqkv: torch.Tensor, num_heads: int, cache: Kv4Cache, pos
         raise ValueError(f"gqkv must be [{b}, seq, 4 * {h} * {d}] for this cache (num_heads {h})")
     s = gqkv.shape[1]
     if out is None:
-        with _on(stream):
-            gate, q = gqkv.new_empty((b, s, h, d)), gqkv.new_empty((b, h, s, d))
-            k, v = (torch.empty_like(q), torch.empty_like(q)) if keep_kv else (None, None)
+        gate, q, k, v = _made(stream, _split_results, gqkv, b, s, h, d, keep_kv)
         given = ()
     else:
         gate, q, k, v = given = tuple(out)
@@ -221,8 +224,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
         if gate.numel() != q.numel():
             raise ValueError("gate has the wrong size")
     if out is None:
-        with _on(stream):
-            out = q.new_empty((b, s, h, d))
+        out = _made(stream, q.new_empty, (b, s, h, d))
     else:
         _need(out, "out")
         if out.numel() != q.numel():
@@ -232,8 +234,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
         raise ValueError("accumulate needs a cache with weights (kv4_cache(..., track=True))")
     nbytes = kv4_attention_workspace(cache, h, s, accumulate)
     if nbytes and workspace is None:
-        with _on(stream):
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        workspace = _made(stream, torch.empty, nbytes, dtype=torch.uint8, device=q.device)
     elif workspace is not None:
         _need(workspace, "workspace", (torch.uint8,))
         nbytes = workspace.numel()
@@ -274,8 +275,7 @@ def kv4_evict(cache: Kv4Cache, lengths: Offset, budget: int, protect_from: Offse
     length, length_t = _offset(lengths, "lengths", b)
     protect, protect_t = _offset(protect_from, "protect_from", b)
     if new_lengths is None:
-        with _on(stream):
-            new_lengths = cache.positions.new_empty(b)
+        new_lengths = _made(stream, cache.positions.new_empty, b)
     else:
         _need(new_lengths, "new_lengths", (torch.int32,))
         if new_lengths.numel() != b:

@@ -12,7 +12,6 @@ uses them waits for it first and, before it drops them, calls record_stream.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -32,13 +31,13 @@ def _stream(t: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> ctypes.c_vo
     return _vp(s.cuda_stream)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(stream: Optional[torch.cuda.Stream]):
-    """Allocations for a launch on `stream` come from that stream's pool: a block of the
-    current stream's may be in use by kernels that are still queued there."""
-    return _HERE if stream is None else torch.cuda.stream(stream)
+def _made(stream: Optional[torch.cuda.Stream], make, *args, **kwargs):
+    """make(...), a call that allocates for a launch on `stream`: from that stream's pool,
+    since a block of the current stream's may be in use by kernels still queued there."""
+    if stream is None:
+        return make(*args, **kwargs)
+    with torch.cuda.stream(stream):
+        return make(*args, **kwargs)
 
 
 def _launch(name: str, tensors, stream: Optional[torch.cuda.Stream], *args) -> None:
@@ -81,9 +80,7 @@ def additive_inject(z_a: torch.Tensor, z_b: torch.Tensor, out: Optional[torch.Te
     _need(z_a, "z_a"); _need(z_b, "z_b")
     if z_a.numel() != z_b.numel():
         raise ValueError("z_a and z_b differ in size")
-    if out is None:
-        with _on(stream):
-            out = torch.empty_like(z_a)
+    out = _made(stream, torch.empty_like, z_a) if out is None else out
     _need(out, "out")
     if out.numel() != z_a.numel():
         raise ValueError("out has the wrong size")
@@ -97,9 +94,7 @@ def swiglu_ffn(gate: torch.Tensor, up: torch.Tensor, out: Optional[torch.Tensor]
     _need(gate, "gate"); _need(up, "up")
     if gate.numel() != up.numel():
         raise ValueError("gate and up differ in size")
-    if out is None:
-        with _on(stream):
-            out = torch.empty_like(gate)
+    out = _made(stream, torch.empty_like, gate) if out is None else out
     _need(out, "out")
     if out.numel() != gate.numel():
         raise ValueError("out has the wrong size")
@@ -124,9 +119,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
         _need(weight, "weight", (x.dtype,))
         if weight.numel() != hidden:
             raise ValueError("weight must have hidden_size elements")
-    if out is None:
-        with _on(stream):
-            out = torch.empty_like(x)
+    out = _made(stream, torch.empty_like, x) if out is None else out
     _need(out, "out", (x.dtype,))
     if out.numel() != x.numel():
         raise ValueError("out has the wrong size")
@@ -150,12 +143,8 @@ def add_rms_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.T
         _need(weight, "weight")
         if weight.numel() != hidden:
             raise ValueError("weight must have hidden_size elements")
-    if residual_out is None:
-        with _on(stream):
-            residual_out = torch.empty_like(x)
-    if normed_out is None:
-        with _on(stream):
-            normed_out = torch.empty_like(x)
+    residual_out = _made(stream, torch.empty_like, x) if residual_out is None else residual_out
+    normed_out = _made(stream, torch.empty_like, x) if normed_out is None else normed_out
     _need(residual_out, "residual_out"); _need(normed_out, "normed_out")
     if residual_out.numel() != x.numel() or normed_out.numel() != x.numel():
         raise ValueError("outputs have the wrong size")
@@ -170,8 +159,7 @@ def rope_table(max_positions: int, head_dim: int, theta: float = 10000.0,
     """fp32 [max_positions, head_dim] table: cos in [:, :hd/2], sin in [:, hd/2:]."""
     if out is None:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        with _on(stream):
-            out = torch.empty((max_positions, head_dim), dtype=torch.float32, device=device)
+        out = _made(stream, torch.empty, (max_positions, head_dim), dtype=torch.float32, device=device)
     _need(out, "out", (torch.float32,))
     if out.numel() != max_positions * head_dim:
         raise ValueError("out has the wrong size")
@@ -227,8 +215,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, embedding_scale: fl
         raise ValueError("table must be [vocab, hidden]")
     vocab, hidden = table.shape
     if out is None:
-        with _on(stream):
-            out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=table.device)
+        out = _made(stream, torch.empty, (*ids.shape, hidden), dtype=table.dtype, device=table.device)
     _need(out, "out")
     if out.numel() != ids.numel() * hidden:
         raise ValueError("out has the wrong size")
@@ -249,11 +236,9 @@ def embed_rms_norm(ids: torch.Tensor, table: torch.Tensor, embedding_scale: floa
     vocab, hidden = table.shape
     shape = (*ids.shape, hidden)
     if hidden_out is None and keep_hidden:
-        with _on(stream):
-            hidden_out = torch.empty(shape, dtype=table.dtype, device=table.device)
+        hidden_out = _made(stream, torch.empty, shape, dtype=table.dtype, device=table.device)
     if normed_out is None:
-        with _on(stream):
-            normed_out = torch.empty(shape, dtype=table.dtype, device=table.device)
+        normed_out = _made(stream, torch.empty, shape, dtype=table.dtype, device=table.device)
     if hidden_out is not None:
         _need(hidden_out, "hidden_out")
     _need(normed_out, "normed_out")
@@ -282,9 +267,8 @@ def split_gqkv_rope(gqkv: torch.Tensor, num_heads: int, position_offset: int = 0
     b, s, w = gqkv.shape
     d = w // (4 * num_heads)
     if out is None:
-        with _on(stream):
-            out = (torch.empty((b, s, num_heads, d), dtype=gqkv.dtype, device=gqkv.device),
-                   *(torch.empty((b, num_heads, s, d), dtype=gqkv.dtype, device=gqkv.device) for _ in range(3)))
+        out = _made(stream, lambda: (gqkv.new_empty((b, s, num_heads, d)),
+                                     *(gqkv.new_empty((b, num_heads, s, d)) for _ in range(3))))
     for t, n in zip(out, ("gate", "q", "k", "v")):
         _need(t, n)
     positions, cache_len = 0, 0
@@ -310,9 +294,7 @@ def gated_attn_output(gate: torch.Tensor, attn_out: torch.Tensor, out: Optional[
     _need(gate, "gate"); _need(attn_out, "attn_out")
     if gate.numel() != attn_out.numel():
         raise ValueError("gate and attn_out differ in size")
-    if out is None:
-        with _on(stream):
-            out = torch.empty_like(attn_out)
+    out = _made(stream, torch.empty_like, attn_out) if out is None else out
     _need(out, "out")
     _launch("hrm_gated_attn_output", (gate, attn_out, out), stream, _ptr(gate), _ptr(attn_out), _ptr(out),
             gate.numel())
@@ -333,8 +315,7 @@ def broadcast_vec(src: torch.Tensor, n_copies: int, out: Optional[torch.Tensor] 
     """out[r, :] = src for r < n_copies (bf16).  src/lib.rs:748-767."""
     _need(src, "src")
     if out is None:
-        with _on(stream):
-            out = torch.empty((n_copies, src.numel()), dtype=src.dtype, device=src.device)
+        out = _made(stream, torch.empty, (n_copies, src.numel()), dtype=src.dtype, device=src.device)
     _need(out, "out")
     if out.numel() != n_copies * src.numel():
         raise ValueError("out has the wrong size")
@@ -353,9 +334,7 @@ def convert_to_bf16(raw: torch.Tensor, dtype: str, out: Optional[torch.Tensor] =
     if raw.numel() % size:
         raise ValueError("raw byte count is not a multiple of the element size")
     n = raw.numel() // size
-    if out is None:
-        with _on(stream):
-            out = torch.empty(n, dtype=torch.bfloat16, device=raw.device)
+    out = _made(stream, torch.empty, n, dtype=torch.bfloat16, device=raw.device) if out is None else out
     _need(out, "out")
     if out.numel() != n:
         raise ValueError("out has the wrong size")
