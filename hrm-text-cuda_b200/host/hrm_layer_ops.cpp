@@ -1,6 +1,7 @@
 // Implementation of the C++ host layer (see hrm_layer_ops.hpp).
 #include "hrm_layer_ops.hpp"
 
+#include <algorithm>
 #include <cstring>
 #include <string>
 
@@ -333,14 +334,22 @@ void HrmLayerOps::kv4_attention(const CudaSlice<bf16>& q, Kv4Cache& cache, const
   if (gate) need(*gate, n, op, "gate");
   int64_t bytes = 0;
   check(hrm_kv4_attention_workspace(&c, (int64_t)num_heads, (int64_t)seq_len, accumulate, &bytes), op);
-  if (workspace_.len() < (size_t)bytes) {  // freeing the old one waits for the calls that use it
-    workspace_ = CudaSlice<uint8_t>();
-    workspace_ = alloc_zero<uint8_t>((size_t)bytes, stream_);
+  uint8_t* workspace = nullptr;
+  size_t workspace_bytes = 0;
+  {
+    const std::lock_guard<std::mutex> lock(workspace_mutex_);
+    const size_t had = workspaces_.empty() ? 0 : workspaces_.back().len();
+    if (had < (size_t)bytes)
+      workspaces_.push_back(alloc_zero<uint8_t>(std::max((size_t)bytes, had + had / 2), stream_));
+    if (!workspaces_.empty()) {
+      workspace = workspaces_.back().device_ptr();
+      workspace_bytes = workspaces_.back().len();
+    }
   }
   check(hrm_kv4_attention(q.device_ptr(), &c, gate ? gate->device_ptr() : nullptr, out.device_ptr(),
                           (int64_t)num_heads, (int64_t)seq_len, (int64_t)cache_offset,
                           per_sequence(cache_offsets, cache.batch, op, "cache_offsets"), (int64_t)prefix_len,
-                          softmax_scale, accumulate, workspace_.device_ptr(), (int64_t)workspace_.len(), stream_),
+                          softmax_scale, accumulate, workspace, (int64_t)workspace_bytes, stream_),
         op);
 }
 

@@ -15,6 +15,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <functional>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -209,7 +210,9 @@ class HrmLayerOps {
   // mha, mha_decode and (with gate) apply_attn_gate over a 4-bit cache: out is [batch,
   // seq_len, num_heads, head_dim].  The layer keeps the workspace between calls; a
   // call that needs more of it than any before allocates it, so make one of the
-  // largest before capturing a graph.
+  // largest before capturing a graph.  A captured call keeps the workspace of its
+  // capture until the layer is destroyed; graphs captured from one layer share it, and
+  // replay one after another.
   void kv4_attention(const CudaSlice<bf16>& q, Kv4Cache& cache, const CudaSlice<bf16>* gate, CudaSlice<bf16>& out,
                      size_t num_heads, size_t seq_len, size_t cache_offset, size_t prefix_len, float softmax_scale,
                      bool accumulate = false, PerSequence cache_offsets = nullptr) const;
@@ -279,7 +282,10 @@ class HrmLayerOps {
   cudaStream_t stream_ = nullptr;
   CudaSlice<float> rope_table_;
   size_t rope_positions_ = 0;
-  mutable CudaSlice<uint8_t> workspace_;  // kv4_attention's; its calls are queued on one stream
+  // kv4_attention's workspace is the last of these; its calls are queued on one stream.  The
+  // outgrown ones, in all at most twice its size, stay: captured graphs hold their addresses.
+  mutable std::vector<CudaSlice<uint8_t>> workspaces_;
+  mutable std::mutex workspace_mutex_;
 };
 
 }  // namespace hrm
