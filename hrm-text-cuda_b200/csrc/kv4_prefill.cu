@@ -356,7 +356,10 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
         // rows that some query must not see: the groups of v that are not finite were read
         // as zeros (before P is handed over: the products free the flags' buffer)
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar(kVFull + (j & 1)), (j >> 1) & 1));
-        if (!ok) break;
+        if (!ok) {
+          tmem_wait_store();  // O's, before its memory is given back
+          break;
+        }
         const uint2* flags = reinterpret_cast<const uint2*>(s_bad[j & 1]);
         uint32_t any = 0;
 #pragma unroll
@@ -395,7 +398,6 @@ __global__ void __launch_bounds__(Pre<D, NQ>::kThreads, 1)
       const uint64_t both = add_f32x2(sum[0], sum[1]);
       l += lo_f32(both) + hi_f32(both);
     }
-    if (!ok) tmem_wait_store();
     const unsigned row = row0 + r;
     const unsigned g = row / a.seq, sq = row - g * a.seq;
     const int64_t head = hk * a.group + g;
