@@ -346,9 +346,12 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 4 : 2)
   // the list could overflow, so that many rows' reads are in flight at once.
   const int per_pass = 32 / lanes, part = lane / lanes;
   // Weight and position go with the row's codes, by its first two lanes, in clusters of CTAs of
-  // 2048 to 4096 rows, else before them, a lane per row (12 heads, 32768 rows on 8
-  // CTAs 25.0 against 27.2 us; 8192 on 4 18.4 and 17.7; 16 x 16 heads of 5000 on one
-  // CTA, whose keys leave no registers for it, 29.9 and 28.0).
+  // 2048 to 4096 rows, else before them, a lane per row (12 heads to a quarter, with
+  // against before: CTAs of 2100 rows, 2, 4 and 8 of them, 20.3 against 20.5 us, 22.4 and 22.7,
+  // 25.6 and 28.2; of 3000 21.5 and 21.7, 23.0 and 24.0, 27.0 and 30.9; of 4000, 2 of
+  // them, 22.2 and 23.0; 32768 rows on 8 to an eighth 24.2 and 26.8.  Smaller CTAs: 8192
+  // on 4 18.4 and 17.7; 16 x 16 heads of 5000 on one CTA, whose keys leave no
+  // registers for it, 29.9 and 28.0).
   const bool with_codes = W == 16 && K == 8 && count > 1;
   const uint32_t* word_from = reinterpret_cast<const uint32_t*>(sub == 0 ? (const void*)weights : positions);
   uint32_t* word_to = reinterpret_cast<uint32_t*>(sub == 0 ? (void*)(a.to.weights + to0) : a.to.positions + to0);

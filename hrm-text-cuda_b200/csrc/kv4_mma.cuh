@@ -10,9 +10,11 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2^x, within 2 ulp; 0
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// sigmoid(g), what the gate of an output multiplies it by, within 4 ulp of fp32: far
-// below the rounding of the bf16 product.  (The exact division is a call of some 40
-// instructions; in a prompt's 128 x 256 outputs per CTA it took as long as 4 tiles.)
+// sigmoid(g), what the gate of an output multiplies it by.  __expf(x) is good to 2 + 1.173 |x|
+// ulp, the reciprocal to 1: within 5 + 1.2 |g| ulp of fp32, 2^-16 of itself where the
+// factor is smallest (g near -87), well below the rounding of the bf16 product, 2^-8.
+// (The exact division is a call of some 40 instructions; in a prompt's 128 x 256
+// outputs per CTA it took as long as 4 tiles.)
 __device__ __forceinline__ float gate_factor(float g) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + __expf(-g)));
@@ -52,11 +54,12 @@ constexpr int64_t kDecodeRows = 8;
 // And up to which it keeps the scores, for a kernel that adds several blocks' up:
 // 4 bytes per row and cache row, against the 160 that the cache has of head_dim 128.
 constexpr int64_t kScoreRows = 16;
-// Query rows of one kv head up to which the decode kernel serves them, in blocks of 8 (12
-// heads of 128, decode kernel against the prompts': 16 rows over 1024 10.1 and 12.2 us, over
-// 8192 20.7 and 24.7, a batch of 8 over 8192 79 and 127; 32 rows 13.6 and 12.1, 38 and
-// 24, 131 and 121: where the two are about even in a batch, its 16 bits of a
-// probability, not 8, decide).
+// Query rows of one kv head up to which the decode kernel serves them, in blocks of 8, with
+// 16 bits of a probability where the prompts' kernel has 8.  12 heads of 128, decode
+// kernel against the prompts': 17 to 24 rows over 1024 11.3 and 12.1 us, a batch of 8 18.9
+// and 21.7, over 8192 29 to 32 and 25, a batch of 8 101 to 103 and 128; 32 rows 13.0 and
+// 12.1, 28 and 21, 37 and 24, 130 and 120.  So a fourth block makes it the slower one, by
+// up to 1.6 times; those rows are served by it for its bits.
 constexpr int64_t kChunkRows = 32;
 
 // What every attention kernel is given.

@@ -24,8 +24,8 @@
 // tile's softmax waits for its own products, P being where S was, so that a tile takes
 // 3400 cycles of softmax and products in turn, the other query tile's in between.
 // Measured (D = 128): 512 queries of 16 heads over 8192 rows 50 us (710 TFLOP/s); 2 x
-// 4096 queries of 12 heads with gate, causal past a prefix of 1000, 125 us (870), and
-// the weights' kernel below 96.  With NQ = 1 a tile takes 3300 cycles: the
+// 4096 queries of 12 heads with gate, causal past a prefix of 1000, 133 us (820), with
+// the weights' kernel below 224.  With NQ = 1 a tile takes 3300 cycles: the
 // stores of the operands and the products share the shared memory's bandwidth (8 x 64 queries
 // of 12 heads over 8192 rows 121 us; k and v filled by 4 warps in turns 135, with one buffer
 // of S 153; codes loaded two tiles ahead 136).

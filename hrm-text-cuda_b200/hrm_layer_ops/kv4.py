@@ -212,7 +212,9 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, cache_offset: Offset, *, gat
     to 1 / sqrt(head_dim); accumulate adds the probabilities to cache.weights.
     workspace: a uint8 tensor of at least kv4_attention_workspace bytes, else one is
     allocated for the call, on the launch's stream.  A sequence with a negative
-    cache_offset whose queries see nothing gives 0.  src/lib.rs:632-704.
+    cache_offset whose queries see nothing gives 0.  A probability has 16 bits in the
+    sum over v for up to 32 query rows of a kv head (heads / kv_heads * s), 8 above.
+    src/lib.rs:632-704.
     """
     _need(q, "q")
     b, hk, _, d = cache.shape

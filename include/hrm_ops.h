@@ -323,10 +323,12 @@ int hrm_split_gqkv_rope_kv4(const void* gqkv, void* gate_out, void* q_out, void*
  *   limit = min(max(cache_offset + s + 1, prefix_len), cache_offset + seq_len, cache_len)
  * (prefix_len 0: causal; more: PrefixLM, as src/kernels/prefixlm_mask.cu:9-41):
  *   p = softmax_j(softmax_scale * q . k_j),  out = sum_j p_j v_j
- * in fp32 with one rounding at the end, times 1 / (1 + exp(-gate)) before that
- * rounding where gate ([batch, seq_len, num_heads, head_dim] bf16) is not NULL.  out
- * is [batch, seq_len, num_heads, head_dim], the layout of the gate and of the
- * output projection.  num_heads is a multiple of kv_heads; query head h reads kv
+ * with scores, softmax and sums in fp32, times 1 / (1 + exp(-gate)) before the one
+ * rounding at the end where gate ([batch, seq_len, num_heads, head_dim] bf16) is not
+ * NULL.  The p_j enter the sum over v with 16 bits for up to 32 query rows of a kv head
+ * (num_heads / kv_heads * seq_len) and as bf16, with 8, above; the sum that they are
+ * divided by, and the weights, have them unrounded.  out is [batch, seq_len,
+ * num_heads, head_dim], the layout of the gate and of the output projection.  num_heads is a multiple of kv_heads; query head h reads kv
  * head h / (num_heads / kv_heads).  A query that sees no row (limit <= 0: a negative
  * cache_offsets entry marks an idle sequence) gives 0.  Rows that a query does not
  * see have no influence on it, whatever they hold.
