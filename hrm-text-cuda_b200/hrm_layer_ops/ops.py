@@ -242,6 +242,8 @@ def embed_rms_norm(ids: torch.Tensor, table: torch.Tensor, embedding_scale: floa
     if hidden_out is not None:
         _need(hidden_out, "hidden_out")
     _need(normed_out, "normed_out")
+    if any(t is not None and t.numel() != ids.numel() * hidden for t in (hidden_out, normed_out)):
+        raise ValueError("outputs have the wrong size")
     if weight is not None:
         _need(weight, "weight")
         if weight.numel() != hidden:
@@ -271,15 +273,20 @@ def split_gqkv_rope(gqkv: torch.Tensor, num_heads: int, position_offset: int = 0
                                      *(gqkv.new_empty((b, num_heads, s, d)) for _ in range(3))))
     for t, n in zip(out, ("gate", "q", "k", "v")):
         _need(t, n)
+        if t.numel() != b * s * num_heads * d:
+            raise ValueError(f"{n} has the wrong size")
     positions, cache_len = 0, 0
     if table is not None:
         _need(table, "table", (torch.float32,))
+        if table.dim() != 2 or table.shape[1] != d:
+            raise ValueError("table must be [positions, head_dim]")
         positions = table.shape[0]
     if (k_cache is None) != (v_cache is None):
         raise ValueError("pass both k_cache and v_cache or neither")
     if k_cache is not None:
         _need(k_cache, "k_cache"); _need(v_cache, "v_cache")
-        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[:2] != (b, num_heads):
+        if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[:2] != (b, num_heads)
+                or k_cache.shape[3] != d):
             raise ValueError("caches must be [batch, heads, cache_len, head_dim]")
         cache_len = k_cache.shape[2]
     _launch("hrm_split_gqkv_rope", (gqkv, *out, table, k_cache, v_cache), stream, _ptr(gqkv),
@@ -296,6 +303,8 @@ def gated_attn_output(gate: torch.Tensor, attn_out: torch.Tensor, out: Optional[
         raise ValueError("gate and attn_out differ in size")
     out = _made(stream, torch.empty_like, attn_out) if out is None else out
     _need(out, "out")
+    if out.numel() != attn_out.numel():
+        raise ValueError("out has the wrong size")
     _launch("hrm_gated_attn_output", (gate, attn_out, out), stream, _ptr(gate), _ptr(attn_out), _ptr(out),
             gate.numel())
     return out
